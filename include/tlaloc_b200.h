@@ -157,6 +157,27 @@ int tlaloc_b200_paged_attention_static(const void* query, int32_t q_dtype, const
                                        int32_t sliding_window, void* stream);
 
 /*
+ * Paged attention of a batch whose rows share prefixes: the keys of row r are those of its prefix and then its own,
+ *   out[r, h] = sum_i e^{s_i} v_i / sum_i e^{s_i},  s_i = scale q[r, h] . k_i
+ * A prefix's keys and values are read once for all of its rows, on the tensor cores where the sizes allow it.
+ *   prefix_tables  device i32 [G, max_prefix_blocks], prefix_lens device i32 [G] (0: none of it; clamped into the table)
+ *   row_starts     device i32 [G + 1], not falling: prefix g is that of rows [row_starts[g], row_starts[g + 1]); rows outside have no prefix
+ *   block_tables, seq_lens   the own positions of each row, as in tlaloc_b200_paged_attention (seq_lens does not count the prefix; 0: none)
+ *   scratch        device memory, 16-byte aligned, contents undefined on entry and exit: tlaloc_b200_shared_prefix_scratch_bytes(...)
+ * query, pools, out, lse (of all the row's keys), dtypes, scale and clamping as in tlaloc_b200_paged_attention.  A row without any key gives zeros (and lse -inf).
+ * Results carry f32 accuracy where out is F32; for a BF16 out the weights of the prefix's keys may be rounded to bf16 in front of the product with the values.
+ * Refused in parity mode.
+ */
+size_t tlaloc_b200_shared_prefix_scratch_bytes(int32_t num_rows, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t num_prefixes,
+                                               int32_t max_blocks_per_seq, int32_t block_size);
+int tlaloc_b200_shared_prefix_attention(const void* query, int32_t q_dtype, const void* key_cache, const void* value_cache, int32_t kv_dtype,
+                                        const int32_t* prefix_tables, const int32_t* prefix_lens, const int32_t* row_starts,
+                                        const int32_t* block_tables, const int32_t* seq_lens, void* out, int32_t out_dtype, float* lse,
+                                        void* scratch, size_t scratch_bytes, int32_t num_rows, int32_t num_heads, int32_t head_dim,
+                                        int32_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t num_prefixes,
+                                        int32_t max_prefix_blocks, int32_t max_blocks_per_seq, int32_t num_tables, float scale, void* stream);
+
+/*
  * KV_CACHE_WRITE (ir/.../KvCacheWriteAttrs.kt:62-159, interpreter
  * DxirInterpreter.kt:2233-2272; XLA scatter form stablehlo/.../StablehloEmitter.kt:4634):
  * row i of new_kv [T, Hkv*D] goes to pool slot slot_mapping[i]; a negative slot
@@ -287,12 +308,48 @@ int tlaloc_b200_rope_kv_write(const float* q, const float* k, const float* v, co
                               int32_t num_slots, int32_t max_pos, int32_t ld_q, int32_t ld_k, int32_t ld_v,
                               void* stream);
 
+/*
+ * A step's queries, keys and values from their projection into attention, in one pass: the norm of every query and key head, the rotation of its first
+ * rot_dims channels, and the append of keys and values to the paged pools.
+ *   y = x * rsqrt(mean(x^2) + eps) * gain over the head's channels (q_gain, k_gain f32 [head_dim], or both NULL: no norm; values are never normed)
+ *   (y_a, y_b) <- (y_a c - y_b s, y_b c + y_a s) for the channel pairs (i, i + rot_dims / 2), or (2i, 2i + 1) with `interleaved`, i < rot_dims / 2
+ *   q, k, v       [T, H, hd], [T, Hkv, hd], [T, Hkv, hd], x_dtype F32 | BF16, rows ld_q, ld_k, ld_v elements apart: they may be column blocks of one projection
+ *   positions     i32 [T], clamped into [0, max_pos)
+ *   cos, sin      f32 [max_pos, rot_dims / 2] (a scaling's magnitude multiplied in); may be NULL for rot_dims 0
+ *   slot_mapping  i32 [T]: the pool row of each token's key and value; negative ones, and ones past num_slots, are not written.  Of tokens that name the same
+ *                 slot one's rows stay, and which one's is not said
+ *   q_out         [T, H, hd] F32 | BF16, contiguous
+ *   pools         [num_slots, Hkv, hd] F32 | BF16 | F8E4M3FN, narrowed as KV_CACHE_WRITE narrows
+ * Arithmetic is f32, each result rounded once at the end.  No output may overlap an input or another output (refused).
+ */
+int tlaloc_b200_norm_rope_kv_write(const void* q, int64_t ld_q, const void* k, int64_t ld_k, const void* v, int64_t ld_v, int32_t x_dtype,
+                                   const float* q_gain, const float* k_gain, float eps, const int32_t* positions, const float* cos_table,
+                                   const float* sin_table, const int32_t* slot_mapping, void* q_out, int32_t q_out_dtype, void* key_cache,
+                                   void* value_cache, int32_t kv_dtype, int32_t num_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                   int32_t rot_dims, int32_t interleaved, int32_t num_slots, int32_t max_pos, void* stream);
+
 /* SwiGLU (HfDecoderGraph.kt:979-988): silu(gate) * up; gate/up f32 with row stride `ld`, out F32 | BF16 [rows, n]. */
 int tlaloc_b200_swiglu(const float* gate, const float* up, int32_t ld, void* out, int32_t out_dtype, int32_t rows,
                        int32_t n, void* stream);
 
 /* Greedy NEXT_TOKEN (DxirInterpreter.kt:2414-2426; triton/kernels/sample.cu greedy arm): first index of the maximum. */
 int tlaloc_b200_argmax(const float* logits, int32_t* out, int32_t rows, int32_t n, void* stream);
+
+/*
+ * One token drawn from each row of logits [rows, n] (F32 | BF16, rows ld elements apart):
+ *   w_i = exp((x_i - max x) / temperature)
+ *   kept are: the top_k largest (0 or less, or n and more: all); of these, best first, each whose betters hold less than top_p of the mass of the top_k (1 and more: all;
+ *   the first one always); of these the ones with w >= min_p (0 and less: all; 1 and more: those equal to the largest).  Equal values rank by index
+ *   token = the first index whose running sum of kept w, in index order, exceeds u * their whole sum
+ *   uniforms      f32 [rows]: u in [0, 1); other values count as the nearer end, NaN as 0
+ *   temperature, top_k, top_p, min_p   per-row settings (f32, i32, f32, f32 [rows]); where one is NULL its *_all value holds for every row
+ *   out           i32 [rows]
+ * A temperature that is not above 0 takes the first of the largest (tlaloc_b200_argmax).  -infinity and NaN are never drawn; where a row holds nothing else its token
+ * is 0.  Where it holds +infinity one of these is drawn.  Weights and sums are f64, in a fixed order: the same inputs give the same token.
+ */
+int tlaloc_b200_sample(const void* logits, int64_t ld, int32_t dtype, const float* uniforms, const float* temperature, const int32_t* top_k,
+                       const float* top_p, const float* min_p, float temperature_all, int32_t top_k_all, float top_p_all, float min_p_all,
+                       int32_t* out, int32_t rows, int32_t n, void* stream);
 
 /* A step's inputs from one buffer into their own: the counts[0] values at packed go to dst[0], the counts[1] after them to dst[1], and so on
  * (1 to 16 segments).  packed and the dst[i] are device memory, the arrays dst and counts host memory, read before the call returns. */

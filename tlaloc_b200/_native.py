@@ -62,8 +62,12 @@ _SIGNATURES = {
     "tlaloc_b200_rmsnorm": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i32, _i32, _f32, _vp]),
     "tlaloc_b200_rmsnorm_planes": (ctypes.c_int, [_vp, _vp, _vp, _vp, _sz, _i32, _i32, _f32, _vp]),
     "tlaloc_b200_rope_kv_write": (ctypes.c_int, [_vp] * 8 + [_i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "tlaloc_b200_norm_rope_kv_write": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _vp, _f32] + [_vp] * 5 + [_i32, _vp, _vp] + [_i32] * 9 + [_vp]),
+    "tlaloc_b200_shared_prefix_scratch_bytes": (_sz, [_i32] * 7),
+    "tlaloc_b200_shared_prefix_attention": (ctypes.c_int, [_vp, _i32, _vp, _vp, _i32] + [_vp] * 6 + [_i32, _vp, _vp, _sz] + [_i32] * 10 + [_f32, _vp]),
     "tlaloc_b200_swiglu": (ctypes.c_int, [_vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp]),
     "tlaloc_b200_argmax": (ctypes.c_int, [_vp, _vp, _i32, _i32, _vp]),
+    "tlaloc_b200_sample": (ctypes.c_int, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _f32, _i32, _f32, _f32, _vp, _i32, _i32, _vp]),
     "tlaloc_b200_unpack_i32": (ctypes.c_int, [_vp, _vp, _vp, _i32, _vp]),
     "tlaloc_b200_dense_gemm": (ctypes.c_int, [ctypes.POINTER(DenseProblem), _i32, _i32, _i32, _i32, _vp]),
     "tlaloc_b200_rmsnorm_pair": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _f32, _vp]),

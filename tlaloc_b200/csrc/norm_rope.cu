@@ -1,0 +1,180 @@
+// Queries, keys and values on their way from a projection to attention (include/tlaloc_b200.h, tlaloc_b200_norm_rope_kv_write): the norm of every query
+// and key head, the rotation of its first channels, and the append of keys and values to the paged pools, in one read and one write.
+//
+//   y = x * rsqrt(mean(x^2) + eps) * gain            over the channels of one head (left out without gains)
+//   (y_a, y_b) <- (y_a c - y_b s, y_b c + y_a s)      for the pairs of the first `rot` channels: (i, i + rot / 2), or (2i, 2i + 1)
+//
+// Bound by HBM: a head's 8 operations a value are nothing beside its 4 to 8 bytes.
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace tlaloc_b200 {
+namespace {
+
+struct NormRopeArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t ld_q, ld_k, ld_v;
+  const float* q_gain;
+  const float* k_gain;
+  const int* positions;
+  const float* cos_t;
+  const float* sin_t;
+  const int* slots;
+  void* q_out;
+  void* kc;
+  void* vc;
+  int T, H, Hkv, D, rot, interleaved, num_slots, max_pos, faithful;
+  float eps;
+};
+
+// Head slot h of a token: a query head, then the key heads, then the value heads.  Where it is read, where it goes (null: nowhere), and what is done with it.
+template <typename XT, typename QT, typename KVT>
+struct HeadSlot {
+  const XT* src;
+  QT* q_dst;
+  KVT* kv_dst;
+  const float* gain;
+  bool rotate;
+  __device__ __forceinline__ HeadSlot(const NormRopeArgs& a, int t, int h, int slot) : src(nullptr), q_dst(nullptr), kv_dst(nullptr), gain(nullptr), rotate(true)
+  {
+    if (h < a.H) {
+      src = static_cast<const XT*>(a.q) + t * a.ld_q + static_cast<int64_t>(h) * a.D;
+      q_dst = static_cast<QT*>(a.q_out) + (static_cast<int64_t>(t) * a.H + h) * a.D;
+      gain = a.q_gain;
+      return;
+    }
+    h -= a.H;
+    const bool value = h >= a.Hkv;
+    if (value) h -= a.Hkv;
+    rotate = !value;
+    gain = value ? nullptr : a.k_gain;
+    src = static_cast<const XT*>(value ? a.v : a.k) + t * (value ? a.ld_v : a.ld_k) + static_cast<int64_t>(h) * a.D;
+    if (slot >= 0 && slot < a.num_slots) kv_dst = static_cast<KVT*>(value ? a.vc : a.kc) + (static_cast<int64_t>(slot) * a.Hkv + h) * a.D;  // else padding: no write
+  }
+};
+
+// Any sizes and strides: a warp per (token, head slot), elements 32 apart.  In parity mode one lane sums the squares in index order, as the interpreter
+// evaluates the norm's nodes (DxirInterpreter.kt:567-572,1791-1807).
+constexpr int kPlainWarps = 8;
+template <typename XT, typename QT, typename KVT>
+__global__ void __launch_bounds__(32 * kPlainWarps) NormRopePlain(const __grid_constant__ NormRopeArgs a)
+{
+  GridDependencySync();
+  const int t = blockIdx.x, h = blockIdx.y * kPlainWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (h >= a.H + 2 * a.Hkv) return;
+  const HeadSlot<XT, QT, KVT> s(a, t, h, __ldg(a.slots + t));
+  if (s.q_dst == nullptr && s.kv_dst == nullptr) return;
+  float rsq = 1.f;
+  if (s.gain != nullptr) {
+    float sum = 0.f;
+    if (a.faithful) {
+      if (lane == 0)
+        for (int j = 0; j < a.D; ++j) sum = __fadd_rn(sum, __fmul_rn(ToF32(s.src[j]), ToF32(s.src[j])));
+      sum = __shfl_sync(0xffffffffu, sum, 0);
+    } else {
+      for (int j = lane; j < a.D; j += 32) sum = fmaf(ToF32(s.src[j]), ToF32(s.src[j]), sum);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    rsq = static_cast<float>(1.0 / sqrt(static_cast<double>(__fadd_rn(__fdiv_rn(sum, static_cast<float>(a.D)), a.eps))));
+  }
+  const int half = a.rot >> 1, pos = min(max(__ldg(a.positions + t), 0), a.max_pos - 1);
+  const float* c = a.cos_t + static_cast<int64_t>(pos) * half;
+  const float* sn = a.sin_t + static_cast<int64_t>(pos) * half;
+  auto normed = [&](int j) {
+    const float x = ToF32(s.src[j]);
+    return s.gain != nullptr ? __fmul_rn(__fmul_rn(x, rsq), __ldg(s.gain + j)) : x;
+  };
+  for (int j = lane; j < a.D; j += 32) {
+    float y = normed(j);
+    if (s.rotate && j < a.rot) {
+      const bool second = a.interleaved ? (j & 1) != 0 : j >= half;
+      const int i = a.interleaved ? j >> 1 : (second ? j - half : j);
+      const float other = normed(a.interleaved ? j ^ 1 : (second ? j - half : j + half));
+      y = __fadd_rn(__fmul_rn(y, __ldg(c + i)), __fmul_rn(second ? other : -other, __ldg(sn + i)));
+    }
+    if (s.q_dst != nullptr) s.q_dst[j] = FromF32<QT>(y);
+    else s.kv_dst[j] = FromF32<KVT>(y);
+  }
+}
+
+template <typename XT, typename QT, typename KVT>
+cudaError_t LaunchNormRope(const NormRopeArgs& a, cudaStream_t st)
+{
+  const dim3 grid(a.T, (a.H + 2 * a.Hkv + kPlainWarps - 1) / kPlainWarps);
+  return LaunchChained(NormRopePlain<XT, QT, KVT>, grid, 32 * kPlainWarps, 0, st, a);
+}
+template <typename XT, typename QT>
+cudaError_t LaunchByPool(const NormRopeArgs& a, int kv_dtype, cudaStream_t st)
+{
+  switch (kv_dtype) {
+    case TLALOC_B200_F32: return LaunchNormRope<XT, QT, float>(a, st);
+    case TLALOC_B200_BF16: return LaunchNormRope<XT, QT, __nv_bfloat16>(a, st);
+    default: return LaunchNormRope<XT, QT, __nv_fp8_e4m3>(a, st);
+  }
+}
+
+// True if the two ranges of bytes have any in common.
+bool Overlap(const void* a, size_t an, const void* b, size_t bn)
+{
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + bn && y < x + an;
+}
+
+}  // namespace
+}  // namespace tlaloc_b200
+
+using namespace tlaloc_b200;
+
+extern "C" int tlaloc_b200_norm_rope_kv_write(const void* q, int64_t ld_q, const void* k, int64_t ld_k, const void* v, int64_t ld_v, int32_t x_dtype,
+                                              const float* q_gain, const float* k_gain, float eps, const int32_t* positions, const float* cos_table,
+                                              const float* sin_table, const int32_t* slot_mapping, void* q_out, int32_t q_out_dtype, void* key_cache,
+                                              void* value_cache, int32_t kv_dtype, int32_t num_tokens, int32_t num_heads, int32_t num_kv_heads,
+                                              int32_t head_dim, int32_t rot_dims, int32_t interleaved, int32_t num_slots, int32_t max_pos, void* stream)
+{
+  const char* op = "NORM_ROPE_KV_WRITE";
+  if (!q || !k || !v || !positions || !slot_mapping || !q_out || !key_cache || !value_cache || (rot_dims > 0 && (!cos_table || !sin_table))) {
+    return Fail(kInvalid, "%s: a required device pointer is null", op);
+  }
+  if (!IsFloatType(x_dtype) || !IsFloatType(q_out_dtype) || !IsPoolType(kv_dtype)) {
+    return Fail(kInvalid, "%s: q, k, v and q_out must be f32 or bf16, the pools f32, bf16 or f8e4m3fn", op);
+  }
+  if (num_tokens < 0 || num_heads < 1 || num_kv_heads < 1 || head_dim < 1 || num_slots < 1 || max_pos < 1) return Fail(kInvalid, "%s: bad sizes", op);
+  if (static_cast<int64_t>(num_heads) + 2ll * num_kv_heads > 65535) return Fail(kUnsupported, "%s: more than 65535 heads", op);
+  if (rot_dims < 0 || rot_dims % 2 != 0 || rot_dims > head_dim) {
+    return Fail(kInvalid, "%s: %d of %d channels cannot be rotated in pairs", op, rot_dims, head_dim);
+  }
+  if ((q_gain == nullptr) != (k_gain == nullptr)) return Fail(kInvalid, "%s: queries and keys have gains both or neither", op);
+  if (q_gain != nullptr && !(eps >= 0.f && eps < 3.0e38f)) return Fail(kInvalid, "%s: eps must be finite and not negative", op);
+  const int64_t q_row = static_cast<int64_t>(num_heads) * head_dim, kv_row = static_cast<int64_t>(num_kv_heads) * head_dim;
+  if (ld_q < q_row || ld_k < kv_row || ld_v < kv_row) return Fail(kInvalid, "%s: a row stride is shorter than its row", op);
+  if (num_tokens == 0) return kOk;
+  // Heads are read while others are written: no output may lie on an input, or on another output.
+  const int64_t last = num_tokens - 1;
+  const size_t xb = DtypeBytes(x_dtype), pool_bytes = static_cast<size_t>(num_slots) * kv_row * DtypeBytes(kv_dtype);
+  const size_t out_bytes = static_cast<size_t>(num_tokens) * q_row * DtypeBytes(q_out_dtype);
+  const struct { const void* at; size_t n; } ins[3] = {{q, (last * ld_q + q_row) * xb}, {k, (last * ld_k + kv_row) * xb}, {v, (last * ld_v + kv_row) * xb}},
+                                             outs[3] = {{q_out, out_bytes}, {key_cache, pool_bytes}, {value_cache, pool_bytes}};
+  for (int i = 0; i < 3; ++i) {
+    for (int j = 0; j < 3; ++j) {
+      if (Overlap(ins[j].at, ins[j].n, outs[i].at, outs[i].n) || (j < i && Overlap(outs[j].at, outs[j].n, outs[i].at, outs[i].n))) {
+        return Fail(kInvalid, "%s: an output overlaps an input or another output", op);
+      }
+    }
+  }
+  const NormRopeArgs a = {q, k, v, ld_q, ld_k, ld_v, q_gain, k_gain, positions, cos_table, sin_table, slot_mapping, q_out, key_cache, value_cache,
+                          num_tokens, num_heads, num_kv_heads, head_dim, rot_dims, interleaved != 0 ? 1 : 0, num_slots, max_pos, OrderFaithful() ? 1 : 0, eps};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (x_dtype == TLALOC_B200_F32) {
+    e = q_out_dtype == TLALOC_B200_F32 ? LaunchByPool<float, float>(a, kv_dtype, st) : LaunchByPool<float, __nv_bfloat16>(a, kv_dtype, st);
+  } else {
+    e = q_out_dtype == TLALOC_B200_F32 ? LaunchByPool<__nv_bfloat16, float>(a, kv_dtype, st) : LaunchByPool<__nv_bfloat16, __nv_bfloat16>(a, kv_dtype, st);
+  }
+  if (e != cudaSuccess) return CudaFail("NORM_ROPE_KV_WRITE launch", e);
+  CountLaunches(1);
+  return kOk;
+}

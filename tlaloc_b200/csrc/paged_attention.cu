@@ -1605,15 +1605,15 @@ extern "C" size_t tlaloc_b200_paged_attention_scratch_bytes(int32_t num_rows, in
   return sizeof(float) * static_cast<size_t>(splits) * num_rows * num_heads * (head_dim + 2);
 }
 
-extern "C" int tlaloc_b200_paged_attention(const void* query, int32_t q_dtype, const void* key_cache,
-                                           const void* value_cache, int32_t kv_dtype, const int32_t* block_tables,
-                                           const int32_t* seq_lens, const int32_t* keep, int32_t keep_chunks,
-                                           void* out, int32_t out_dtype, float* lse, float* scratch, int32_t splits,
-                                           int32_t num_rows, int32_t num_heads, int32_t head_dim, int32_t num_blocks,
-                                           int32_t block_size, int32_t num_kv_heads, int32_t max_blocks_per_seq,
-                                           int32_t num_tables, float scale, int32_t sliding_window, void* stream)
+namespace tlaloc_b200 {
+namespace {
+
+// The operator's checks, and the parameters that follow from its operands (all but the slices).
+int ParseCall(const char* op, const void* query, int32_t q_dtype, const void* key_cache, const void* value_cache, int32_t kv_dtype, const int32_t* block_tables,
+              const int32_t* seq_lens, const int32_t* keep, int32_t keep_chunks, void* out, int32_t out_dtype, float* lse, float* scratch, int32_t splits,
+              int32_t num_rows, int32_t num_heads, int32_t head_dim, int32_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t max_blocks_per_seq,
+              int32_t num_tables, float scale, int32_t sliding_window, PaParams* params)
 {
-  const char* op = "PAGED_ATTENTION";
   if (!query || !key_cache || !value_cache || !block_tables || !seq_lens || !out || !scratch) {
     return Fail(kInvalid, "%s: a required device pointer is null", op);
   }
@@ -1650,7 +1650,7 @@ extern "C" int tlaloc_b200_paged_attention(const void* query, int32_t q_dtype, c
   if (splits < 1) return Fail(kInvalid, "%s: scratch must hold at least one slice", op);
   if (head_dim > 256) return Fail(kUnsupported, "%s: headDim %d > 256", op, head_dim);
 
-  PaParams p;
+  PaParams& p = *params;
   p.q = query;
   p.kc = key_cache;
   p.vc = value_cache;
@@ -1676,10 +1676,101 @@ extern "C" int tlaloc_b200_paged_attention(const void* query, int32_t q_dtype, c
   p.keep_chunk = keep ? ctx / keep_chunks : 1;
   p.bs_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
   p.scale = scale;
+  return kOk;
+}
 
+// The slice kernels of a parsed call: fills in the slices that they use.
+int LaunchSlices(const char* op, PaParams& p, int32_t q_dtype, int32_t kv_dtype, int32_t splits, cudaStream_t st)
+{
+  const int ctx = p.M * p.bs;
+  // The tensor-core kernel copies K/V rows in 16-byte pieces: pools that start off a 16-byte boundary (a slice of a
+  // larger allocation at an odd element) take the generic kernel, which has no alignment needs.
+  // $TLALOC_B200_PA_F8_GENERIC=1 sends e4m3fn pools to the generic kernel (a debugging aid).
+  static const bool f8_generic = [] {
+    const char* v = std::getenv("TLALOC_B200_PA_F8_GENERIC");
+    return v != nullptr && v[0] == '1';
+  }();
+  const bool f8 = kv_dtype == TLALOC_B200_F8E4M3FN;
+  const bool mma = (kv_dtype == TLALOC_B200_BF16 || (f8 && !f8_generic)) && (p.D == 64 || p.D == 128) && p.NQ <= kMmaQ &&
+                   p.keep == nullptr && (f8 ? p.bs >= 16 : p.bs >= 8) && Aligned16(p.kc) && Aligned16(p.vc);
+  // Slice length: the preferred one (tensor-core kernel) or 256, stretched until `splits` slices cover the context.
+  const bool from_window = p.window > 0 && p.window < ctx && p.rpt == 1;  // rows that share a table have windows in different places: all slices are launched for them
+  const int seen = from_window ? p.window : ctx;
+  int slice = mma ? PreferredSlice(seen, from_window, p.Tb, p.Hkv, f8) : 256;
+  if (static_cast<int64_t>(slice) * splits < ctx) slice = (ctx + splits - 1) / splits;
+  if (mma) slice = std::min((slice + 15) / 16 * 16, 8192);
+  if (static_cast<int64_t>(slice) * splits < ctx) {
+    return Fail(kInvalid, "%s: scratch holds %d slices, too few for %d positions", op, splits, ctx);
+  }
+  p.slice = slice;
+  p.S = (ctx + slice - 1) / slice;
+  p.grid = from_window ? std::min(p.S, (p.window + slice - 2) / slice + 1) : p.S;
+
+  cudaError_t e = cudaSuccess;
+  if (mma) {
+    e = PreparePagedAttentionKernels();
+    if (e != cudaSuccess) return CudaFail("PAGED_ATTENTION set-up", e);
+    if (f8) {
+      if (q_dtype == TLALOC_B200_BF16) e = p.D == 64 ? LaunchMmaF8<__nv_bfloat16, 64>(p, st) : LaunchMmaF8<__nv_bfloat16, 128>(p, st);
+      else e = p.D == 64 ? LaunchMmaF8<float, 64>(p, st) : LaunchMmaF8<float, 128>(p, st);
+    } else if (q_dtype == TLALOC_B200_BF16) {
+      e = p.D == 64 ? LaunchMma<__nv_bfloat16, 64>(p, st) : LaunchMma<__nv_bfloat16, 128>(p, st);
+    } else {
+      e = p.D == 64 ? LaunchMma<float, 64>(p, st) : LaunchMma<float, 128>(p, st);
+    }
+  } else if (q_dtype == TLALOC_B200_F32 && kv_dtype == TLALOC_B200_F32) {
+    e = LaunchGeneric<float, float>(p, st);
+  } else if (q_dtype == TLALOC_B200_F32 && kv_dtype == TLALOC_B200_BF16) {
+    e = LaunchGeneric<float, __nv_bfloat16>(p, st);
+  } else if (q_dtype == TLALOC_B200_F32) {
+    e = LaunchGeneric<float, __nv_fp8_e4m3>(p, st);
+  } else if (kv_dtype == TLALOC_B200_F32) {
+    e = LaunchGeneric<__nv_bfloat16, float>(p, st);
+  } else if (kv_dtype == TLALOC_B200_BF16) {
+    e = LaunchGeneric<__nv_bfloat16, __nv_bfloat16>(p, st);
+  } else {
+    e = LaunchGeneric<__nv_bfloat16, __nv_fp8_e4m3>(p, st);
+  }
+  if (e != cudaSuccess) return CudaFail("PAGED_ATTENTION slice launch", e);
+  return kOk;
+}
+
+}  // namespace
+
+int LaunchPagedSlices(const char* op, const void* query, int32_t q_dtype, const void* key_cache, const void* value_cache, int32_t kv_dtype,
+                      const int32_t* block_tables, const int32_t* seq_lens, float* records, int32_t splits, int32_t num_rows, int32_t num_heads, int32_t head_dim,
+                      int32_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t max_blocks_per_seq, int32_t num_tables, float scale, cudaStream_t st,
+                      int32_t* slice, int32_t* slices)
+{
+  PaParams p;
+  int rc = ParseCall(op, query, q_dtype, key_cache, value_cache, kv_dtype, block_tables, seq_lens, nullptr, 0, records, TLALOC_B200_F32, nullptr, records, splits,
+                     num_rows, num_heads, head_dim, num_blocks, block_size, num_kv_heads, max_blocks_per_seq, num_tables, scale, 0, &p);
+  if (rc == kOk) rc = LaunchSlices(op, p, q_dtype, kv_dtype, splits, st);
+  if (rc != kOk) return rc;
+  *slice = p.slice;
+  *slices = p.S;
+  CountLaunches(1);
+  return kOk;
+}
+
+}  // namespace tlaloc_b200
+
+extern "C" int tlaloc_b200_paged_attention(const void* query, int32_t q_dtype, const void* key_cache,
+                                           const void* value_cache, int32_t kv_dtype, const int32_t* block_tables,
+                                           const int32_t* seq_lens, const int32_t* keep, int32_t keep_chunks,
+                                           void* out, int32_t out_dtype, float* lse, float* scratch, int32_t splits,
+                                           int32_t num_rows, int32_t num_heads, int32_t head_dim, int32_t num_blocks,
+                                           int32_t block_size, int32_t num_kv_heads, int32_t max_blocks_per_seq,
+                                           int32_t num_tables, float scale, int32_t sliding_window, void* stream)
+{
+  const char* op = "PAGED_ATTENTION";
+  PaParams p;
+  int rc = ParseCall(op, query, q_dtype, key_cache, value_cache, kv_dtype, block_tables, seq_lens, keep, keep_chunks, out, out_dtype, lse, scratch, splits,
+                     num_rows, num_heads, head_dim, num_blocks, block_size, num_kv_heads, max_blocks_per_seq, num_tables, scale, sliding_window, &p);
+  if (rc != kOk) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (OrderFaithful()) {  // parity mode: the interpreter's walk, straight into out (no slices, no scratch use)
-    const int span = sliding_window > 0 ? std::min(sliding_window, ctx) : ctx;
+    const int ctx = p.M * p.bs, span = sliding_window > 0 ? std::min(sliding_window, ctx) : ctx;
     if (span > kFaithfulMaxCtx) {
       return Fail(kUnsupported, "%s: parity mode holds a row's scores on chip, at most %d positions (got %d)", op, kFaithfulMaxCtx, span);
     }
@@ -1696,55 +1787,9 @@ extern "C" int tlaloc_b200_paged_attention(const void* query, int32_t q_dtype, c
     CountLaunches(1);
     return kOk;
   }
-  // The tensor-core kernel copies K/V rows in 16-byte pieces: pools that start off a 16-byte boundary (a slice of a
-  // larger allocation at an odd element) take the generic kernel, which has no alignment needs.
-  // $TLALOC_B200_PA_F8_GENERIC=1 sends e4m3fn pools to the generic kernel (a debugging aid).
-  static const bool f8_generic = [] {
-    const char* v = std::getenv("TLALOC_B200_PA_F8_GENERIC");
-    return v != nullptr && v[0] == '1';
-  }();
-  const bool f8 = kv_dtype == TLALOC_B200_F8E4M3FN;
-  const bool mma = (kv_dtype == TLALOC_B200_BF16 || (f8 && !f8_generic)) && (head_dim == 64 || head_dim == 128) && p.NQ <= kMmaQ &&
-                   keep == nullptr && (f8 ? block_size >= 16 : block_size >= 8) && Aligned16(key_cache) && Aligned16(value_cache);
-  // Slice length: the preferred one (tensor-core kernel) or 256, stretched until `splits` slices cover the context.
-  const bool from_window = sliding_window > 0 && sliding_window < ctx && p.rpt == 1;  // rows that share a table have windows in different places: all slices are launched for them
-  const int seen = from_window ? sliding_window : ctx;
-  int slice = mma ? PreferredSlice(seen, from_window, num_tables, num_kv_heads, f8) : 256;
-  if (static_cast<int64_t>(slice) * splits < ctx) slice = (ctx + splits - 1) / splits;
-  if (mma) slice = std::min((slice + 15) / 16 * 16, 8192);
-  if (static_cast<int64_t>(slice) * splits < ctx) {
-    return Fail(kInvalid, "%s: scratch holds %d slices, too few for %d positions", op, splits, ctx);
-  }
-  p.slice = slice;
-  p.S = (ctx + slice - 1) / slice;
-  p.grid = from_window ? std::min(p.S, (sliding_window + slice - 2) / slice + 1) : p.S;
-
+  rc = LaunchSlices(op, p, q_dtype, kv_dtype, splits, st);
+  if (rc != kOk) return rc;
   cudaError_t e = cudaSuccess;
-  if (mma) {
-    e = PreparePagedAttentionKernels();
-    if (e != cudaSuccess) return CudaFail("PAGED_ATTENTION set-up", e);
-    if (f8) {
-      if (q_dtype == TLALOC_B200_BF16) e = head_dim == 64 ? LaunchMmaF8<__nv_bfloat16, 64>(p, st) : LaunchMmaF8<__nv_bfloat16, 128>(p, st);
-      else e = head_dim == 64 ? LaunchMmaF8<float, 64>(p, st) : LaunchMmaF8<float, 128>(p, st);
-    } else if (q_dtype == TLALOC_B200_BF16) {
-      e = head_dim == 64 ? LaunchMma<__nv_bfloat16, 64>(p, st) : LaunchMma<__nv_bfloat16, 128>(p, st);
-    } else {
-      e = head_dim == 64 ? LaunchMma<float, 64>(p, st) : LaunchMma<float, 128>(p, st);
-    }
-  } else if (q_dtype == TLALOC_B200_F32 && kv_dtype == TLALOC_B200_F32) {
-    e = LaunchGeneric<float, float>(p, st);
-  } else if (q_dtype == TLALOC_B200_F32 && kv_dtype == TLALOC_B200_BF16) {
-    e = LaunchGeneric<float, __nv_bfloat16>(p, st);
-  } else if (q_dtype == TLALOC_B200_F32) {
-    e = LaunchGeneric<float, __nv_fp8_e4m3>(p, st);
-  } else if (kv_dtype == TLALOC_B200_F32) {
-    e = LaunchGeneric<__nv_bfloat16, float>(p, st);
-  } else if (kv_dtype == TLALOC_B200_BF16) {
-    e = LaunchGeneric<__nv_bfloat16, __nv_bfloat16>(p, st);
-  } else {
-    e = LaunchGeneric<__nv_bfloat16, __nv_fp8_e4m3>(p, st);
-  }
-  if (e != cudaSuccess) return CudaFail("PAGED_ATTENTION slice launch", e);
   const unsigned cgrid = static_cast<unsigned>((p.R * p.H + kCombineThreads / 32 - 1) / (kCombineThreads / 32));
   if (out_dtype == TLALOC_B200_F32) {
     e = p.D <= 64    ? LaunchChained(PaCombine<float, 1>, cgrid, kCombineThreads, 0, st, p)

@@ -1,0 +1,383 @@
+// Attention of a batch whose rows share prefixes (include/tlaloc_b200.h, tlaloc_b200_shared_prefix_attention): a row's keys are those of its prefix, read from
+// pages that all rows of the prefix have in common, and then its own, read from its own pages as in paged attention.
+//
+//   out = sum_i e^{s_i - m} v_i / sum_i e^{s_i - m},  s_i = scale q . k_i,  over the keys of both parts
+//
+// Softmax over a set of keys is the merge of softmaxes over its parts: with {m, l, acc} of every part, out = sum e^{m - M} acc / sum e^{m - M} l.  Three launches:
+//   prefix records   each prefix's keys and values read once for all (row, head) pairs that see them, as matrix products over tiles of pairs and keys
+//   own records      the slice kernels of paged attention (paged_attention.cu)
+//   merge            a warp per (row, head) over the records of both
+#include <algorithm>
+
+#include "shared_prefix.cuh"
+
+namespace tlaloc_b200 {
+namespace {
+
+struct PrefixArgs {
+  PrefixPlan plan;
+  const void* q;
+  const void* kc;
+  const void* vc;
+  const int* tables;  // [G, M]
+  float* records;     // [max_blocks, unit_rows, D + 2]
+  int H, D, bs, M, P;
+  float scale;
+};
+
+// ------------------------------------------------------------------------------------------
+// Any type, head size and page size: f32 FMAs over tiles of 64 pairs x 32 keys in shared memory.
+
+constexpr int kPairs = 64, kTileKeys = 32, kTiledThreads = 256;
+
+// Thread (ty, tx) of 16 x 16: scores of pairs 4 ty .. 4 ty + 3 with keys tx and tx + 16; outputs of the same pairs at channels tx + 16 j, j < NJ.
+template <typename QT, typename KVT, int NJ>
+__global__ void __launch_bounds__(kTiledThreads) PrefixTiled(const __grid_constant__ PrefixArgs a)
+{
+  extern __shared__ __align__(16) float smem[];
+  __shared__ PrefixSegment seg_s;
+  __shared__ int more_s;
+  __shared__ float m_s[kPairs], l_s[kPairs], alpha_s[kPairs];
+  __shared__ long long off_s[kTileKeys];
+  GridDependencySync();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ty = tid >> 4, tx = tid & 15;
+  const int D = a.D, ld = (D + 3) / 4 * 4 + 4;  // rows of q and k: zeros up to a multiple of 4; 4 more for the banks
+  float* qs = smem;                  // [kPairs][ld]
+  float* ks = qs + kPairs * ld;      // [kTileKeys][ld]
+  float* vs = ks + kTileKeys * ld;   // [kTileKeys][ld]
+  float* ps = vs + kTileKeys * ld;   // [kPairs][kTileKeys + 1]
+  const QT* q = static_cast<const QT*>(a.q);
+  const KVT* kc = static_cast<const KVT*>(a.kc);
+  const KVT* vc = static_cast<const KVT*>(a.vc);
+  long long total, run = 0, at = 0, end = 0;
+  if (warp == 0) {
+    run = PrefixRun(a.plan, &total);
+    at = blockIdx.x * run;
+    end = min(at + run, total);
+  }
+  for (;;) {
+    __syncthreads();
+    if (warp == 0) {
+      PrefixSegment s;
+      const bool more = PrefixNext(a.plan, run, end, &at, &s);
+      if (lane == 0) {
+        more_s = more ? 1 : 0;
+        if (more) seg_s = s;
+      }
+    }
+    __syncthreads();
+    if (more_s == 0) return;
+    const PrefixSegment s = seg_s;
+    auto row_of = [&](int pair) { return s.row0 + (s.pair0 + pair) / a.plan.group; };
+    auto head_of = [&](int pair) { return s.kv * a.plan.group + (s.pair0 + pair) % a.plan.group; };
+    for (int i = tid; i < kPairs * ld; i += kTiledThreads) {
+      const int r = i / ld, d = i - r * ld;
+      qs[i] = r < s.pairs && d < D ? ToF32(q[(static_cast<size_t>(row_of(r)) * a.H + head_of(r)) * D + d]) * a.scale : 0.f;
+    }
+    if (tid < kPairs) {
+      m_s[tid] = -INFINITY;
+      l_s[tid] = 0.f;
+    }
+    float acc[4][NJ];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i][j] = 0.f;
+    for (int t = s.tile0; t < s.tile1; ++t) {
+      const int key0 = t * kTileKeys, n = min(kTileKeys, s.len - key0);
+      __syncthreads();
+      if (tid < n) {
+        const int pos = key0 + tid;
+        const int page = min(max(__ldg(a.tables + static_cast<size_t>(s.index) * a.M + pos / a.bs), 0), a.P - 1);
+        off_s[tid] = ((static_cast<long long>(page) * a.bs + pos % a.bs) * a.plan.Hkv + s.kv) * D;
+      }
+      __syncthreads();
+      for (int i = tid; i < kTileKeys * ld; i += kTiledThreads) {  // positions past the end are zeros: 0 times whatever a page holds there must stay 0
+        const int r = i / ld, d = i - r * ld;
+        const bool live = r < n && d < D;
+        ks[i] = live ? ToF32(kc[off_s[r] + d]) : 0.f;
+        vs[i] = live ? ToF32(vc[off_s[r] + d]) : 0.f;
+      }
+      __syncthreads();
+      float sc[4][2] = {};
+      for (int d = 0; d < ld - 4; d += 4) {
+        const float4 k0 = *reinterpret_cast<const float4*>(ks + tx * ld + d), k1 = *reinterpret_cast<const float4*>(ks + (tx + 16) * ld + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 x = *reinterpret_cast<const float4*>(qs + (ty * 4 + i) * ld + d);
+          sc[i][0] = fmaf(x.x, k0.x, fmaf(x.y, k0.y, fmaf(x.z, k0.z, fmaf(x.w, k0.w, sc[i][0]))));
+          sc[i][1] = fmaf(x.x, k1.x, fmaf(x.y, k1.y, fmaf(x.z, k1.z, fmaf(x.w, k1.w, sc[i][1]))));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ps[(ty * 4 + i) * (kTileKeys + 1) + tx] = tx < n ? sc[i][0] : -INFINITY;
+        ps[(ty * 4 + i) * (kTileKeys + 1) + tx + 16] = tx + 16 < n ? sc[i][1] : -INFINITY;
+      }
+      __syncthreads();
+      // The running maximum and sum of a pair: a warp takes eight pairs, a lane one key.
+      for (int r = warp * 8; r < warp * 8 + 8; ++r) {
+        const float x = ps[r * (kTileKeys + 1) + lane];
+        float top = x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float before = m_s[r], now = fmaxf(before, top);
+        const float ref = now == -INFINITY ? 0.f : now;  // scores that are all -infinity weigh nothing
+        const float e = expf(x - ref);
+        float sum = e;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        ps[r * (kTileKeys + 1) + lane] = e;
+        __syncwarp();
+        if (lane == 0) {
+          const float alpha = expf(before - ref);
+          alpha_s[r] = alpha;
+          l_s[r] = l_s[r] * alpha + sum;
+          m_s[r] = now;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float alpha = alpha_s[ty * 4 + i];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] *= alpha;
+      }
+      for (int k = 0; k < n; ++k) {
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = ps[(ty * 4 + i) * (kTileKeys + 1) + k];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const int d = tx + 16 * j;
+          const float v = d < D ? vs[k * ld + d] : 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i][j] = fmaf(w[i], v, acc[i][j]);
+        }
+      }
+    }
+    if (s.block < 0) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = ty * 4 + i;
+      if (r >= s.pairs) continue;
+      float* rec = a.records + (static_cast<size_t>(s.block) * kPairs + r) * (D + 2);
+      if (tx == 0) {
+        rec[0] = m_s[r];
+        rec[1] = l_s[r];
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int d = tx + 16 * j;
+        if (d < D) rec[2 + d] = acc[i][j];
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// The merge.
+
+struct MergeArgs {
+  PrefixPlan plan;
+  const float* prefix;  // [max_blocks, unit_rows, D + 2]
+  const float* own;     // [slices, R, H, D + 2]
+  const int* lens;      // [R], own positions
+  void* out;
+  float* lse;
+  int H, D, max_own, slice, slices;
+};
+
+constexpr int kMergeWarps = 4;
+
+// A warp per (row, head); lane l owns channels l, l + 32, ...  The records in order: the prefix's by CTA, then the own slices; the same order in every run.
+template <typename OT>
+__global__ void __launch_bounds__(32 * kMergeWarps) PrefixMerge(const __grid_constant__ MergeArgs a)
+{
+  GridDependencySync();
+  const int lane = threadIdx.x & 31;
+  const long long rh = static_cast<long long>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5);
+  if (rh >= static_cast<long long>(a.plan.R) * a.H) return;
+  const int row = static_cast<int>(rh / a.H), head = static_cast<int>(rh % a.H), kv = head / a.plan.group;
+  const int own = min((min(max(__ldg(a.lens + row), 0), a.max_own) + a.slice - 1) / a.slice, a.slices);
+  long long total;
+  const long long run = PrefixRun(a.plan, &total);
+  PrefixGroup g;
+  int index, shared = 0;
+  const float* first = nullptr;
+  const size_t step = static_cast<size_t>(a.plan.unit_rows) * (a.D + 2), own_step = static_cast<size_t>(a.plan.R) * a.H * (a.D + 2);
+  if (PrefixFind(a.plan, true, row, &g, &index) && g.tiles > 0) {
+    const int pair = (row - g.row0) * a.plan.group + head % a.plan.group;
+    const long long unit = static_cast<long long>(kv) * g.units + pair / a.plan.unit_rows, work = g.work0 + unit * g.tiles;
+    const long long c0 = work / run, c1 = (work + g.tiles - 1) / run, block = c0 + g.unit0 + unit;
+    if (block + (c1 - c0) < a.plan.max_blocks) {
+      shared = static_cast<int>(c1 - c0 + 1);
+      first = a.prefix + block * step + static_cast<size_t>(pair % a.plan.unit_rows) * (a.D + 2);
+    }
+  }
+  const float* mine = a.own + static_cast<size_t>(rh) * (a.D + 2);
+  const int n = shared + own;
+  auto record = [&](int i) { return i < shared ? first + i * step : mine + (i - shared) * own_step; };
+  float top = -INFINITY;
+  for (int i = lane; i < n; i += 32) top = fmaxf(top, record(i)[0]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float sum = 0.f, acc[8] = {};
+  for (int i = 0; i < n; ++i) {
+    const float* r = record(i);
+    const float w = r[0] == -INFINITY ? 0.f : expf(r[0] - top);
+    if (w == 0.f) continue;
+    sum += w * r[1];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (lane + 32 * j < a.D) acc[j] += w * r[2 + lane + 32 * j];
+  }
+  OT* out = static_cast<OT*>(a.out) + rh * a.D;
+  const bool empty = top == -INFINITY || sum == 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (lane + 32 * j < a.D) out[lane + 32 * j] = FromF32<OT>(empty ? 0.f : acc[j] / sum);
+  if (lane == 0 && a.lse != nullptr) a.lse[rh] = empty ? -INFINITY : top + logf(sum);
+}
+
+// ------------------------------------------------------------------------------------------
+// Host side.
+
+constexpr int kTiledGrid = 2 * 148;
+
+size_t TiledSmem(int D) { return sizeof(float) * ((kPairs + 2 * kTileKeys) * ((D + 3) / 4 * 4 + 4) + kPairs * (kTileKeys + 1)); }
+
+template <typename QT, typename KVT>
+cudaError_t PrepareTiled()
+{
+  const int most = static_cast<int>(TiledSmem(256));
+  cudaError_t e = cudaFuncSetAttribute(PrefixTiled<QT, KVT, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(PrefixTiled<QT, KVT, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(PrefixTiled<QT, KVT, 16>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  return e;
+}
+template <typename QT, typename KVT>
+cudaError_t LaunchTiled(const PrefixArgs& a, cudaStream_t st)
+{
+  const size_t smem = TiledSmem(a.D);
+  return a.D <= 64    ? LaunchChained(PrefixTiled<QT, KVT, 4>, a.plan.grid, kTiledThreads, smem, st, a)
+         : a.D <= 128 ? LaunchChained(PrefixTiled<QT, KVT, 8>, a.plan.grid, kTiledThreads, smem, st, a)
+                      : LaunchChained(PrefixTiled<QT, KVT, 16>, a.plan.grid, kTiledThreads, smem, st, a);
+}
+template <typename QT>
+cudaError_t LaunchTiledByPool(const PrefixArgs& a, int kv_dtype, cudaStream_t st)
+{
+  switch (kv_dtype) {
+    case TLALOC_B200_F32: return LaunchTiled<QT, float>(a, st);
+    case TLALOC_B200_BF16: return LaunchTiled<QT, __nv_bfloat16>(a, st);
+    default: return LaunchTiled<QT, __nv_fp8_e4m3>(a, st);
+  }
+}
+
+cudaError_t PrepareSharedPrefix()
+{
+  static OncePerDevice once;
+  return once.Run([](int) {
+    cudaError_t e = PrepareTiled<float, float>();
+    if (e == cudaSuccess) e = PrepareTiled<float, __nv_bfloat16>();
+    if (e == cudaSuccess) e = PrepareTiled<float, __nv_fp8_e4m3>();
+    if (e == cudaSuccess) e = PrepareTiled<__nv_bfloat16, float>();
+    if (e == cudaSuccess) e = PrepareTiled<__nv_bfloat16, __nv_bfloat16>();
+    if (e == cudaSuccess) e = PrepareTiled<__nv_bfloat16, __nv_fp8_e4m3>();
+    return e;
+  });
+}
+KernelSetup g_setup(PrepareSharedPrefix, nullptr);
+
+// Blocks of records that a cut of `grid` runs can use: units of `unit_rows` pairs, at most one part-filled one per prefix and KV head.
+long long RecordBlocks(int rows, int heads, int kv_heads, int prefixes, int unit_rows, int grid)
+{
+  const long long pairs = static_cast<long long>(rows) * (heads / kv_heads);
+  return grid + kv_heads * (pairs / unit_rows + std::min<long long>(prefixes, rows));
+}
+size_t RecordBytes(long long blocks, int unit_rows, int head_dim) { return static_cast<size_t>(blocks) * unit_rows * (head_dim + 2) * sizeof(float); }
+int OwnSlices(int max_blocks, int block_size) { return static_cast<int>((static_cast<long long>(max_blocks) * block_size + 255) / 256); }
+
+}  // namespace
+}  // namespace tlaloc_b200
+
+using namespace tlaloc_b200;
+
+extern "C" size_t tlaloc_b200_shared_prefix_scratch_bytes(int32_t num_rows, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t num_prefixes,
+                                                          int32_t max_blocks_per_seq, int32_t block_size)
+{
+  if (num_rows < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1 || num_prefixes < 1 || max_blocks_per_seq < 1 || block_size < 1) return 0;
+  const size_t records = RecordBytes(RecordBlocks(num_rows, num_heads, num_kv_heads, num_prefixes, kPairs, kTiledGrid), kPairs, head_dim);
+  return records + tlaloc_b200_paged_attention_scratch_bytes(num_rows, num_heads, head_dim, OwnSlices(max_blocks_per_seq, block_size));
+}
+
+extern "C" int tlaloc_b200_shared_prefix_attention(const void* query, int32_t q_dtype, const void* key_cache, const void* value_cache, int32_t kv_dtype,
+                                                   const int32_t* prefix_tables, const int32_t* prefix_lens, const int32_t* row_starts,
+                                                   const int32_t* block_tables, const int32_t* seq_lens, void* out, int32_t out_dtype, float* lse,
+                                                   void* scratch, size_t scratch_bytes, int32_t num_rows, int32_t num_heads, int32_t head_dim,
+                                                   int32_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t num_prefixes,
+                                                   int32_t max_prefix_blocks, int32_t max_blocks_per_seq, int32_t num_tables, float scale, void* stream)
+{
+  const char* op = "SHARED_PREFIX_ATTENTION";
+  if (!prefix_tables || !prefix_lens || !row_starts || !out || !scratch) return Fail(kInvalid, "%s: a required device pointer is null", op);
+  if (!IsFloatType(out_dtype)) return Fail(kInvalid, "%s: out must be f32 or bf16", op);
+  if (num_prefixes < 1 || max_prefix_blocks < 1 || block_size < 1) return Fail(kInvalid, "%s: needs one prefix table or more, of one block or more", op);
+  if (static_cast<int64_t>(max_prefix_blocks) * block_size > (1 << 30)) return Fail(kUnsupported, "%s: a prefix of %lld positions is too long", op, static_cast<long long>(max_prefix_blocks) * block_size);
+  if (OrderFaithful()) return Fail(kUnsupported, "%s: has no parity mode", op);
+  const size_t need = tlaloc_b200_shared_prefix_scratch_bytes(num_rows, num_heads, num_kv_heads, head_dim, num_prefixes, max_blocks_per_seq, block_size);
+  if (scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15) != 0) {
+    return Fail(kInvalid, "%s: scratch must be 16-byte aligned and hold %zu bytes (got %zu)", op, need, scratch_bytes);
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int own_slices = OwnSlices(max_blocks_per_seq, block_size);
+  float* own = static_cast<float*>(scratch);
+  float* records = own + tlaloc_b200_paged_attention_scratch_bytes(num_rows, num_heads, head_dim, own_slices) / sizeof(float);
+  MergeArgs m = {};
+  // The own part first: its checks are those of all the operands that both parts share.
+  int rc = LaunchPagedSlices(op, query, q_dtype, key_cache, value_cache, kv_dtype, block_tables, seq_lens, own, own_slices, num_rows, num_heads, head_dim,
+                             num_blocks, block_size, num_kv_heads, max_blocks_per_seq, num_tables, scale, st, &m.slice, &m.slices);
+  if (rc != kOk) return rc;
+  cudaError_t e = PrepareSharedPrefix();
+  if (e != cudaSuccess) return CudaFail("SHARED_PREFIX_ATTENTION set-up", e);
+  PrefixArgs a = {};
+  a.plan.lens = prefix_lens;
+  a.plan.starts = row_starts;
+  a.plan.G = num_prefixes;
+  a.plan.R = num_rows;
+  a.plan.group = num_heads / num_kv_heads;
+  a.plan.Hkv = num_kv_heads;
+  a.plan.max_len = max_prefix_blocks * block_size;
+  a.plan.unit_rows = kPairs;
+  a.plan.tile = kTileKeys;
+  a.plan.grid = kTiledGrid;
+  a.plan.min_run = 4;
+  a.plan.max_blocks = static_cast<int>(RecordBlocks(num_rows, num_heads, num_kv_heads, num_prefixes, kPairs, kTiledGrid));
+  a.q = query;
+  a.kc = key_cache;
+  a.vc = value_cache;
+  a.tables = prefix_tables;
+  a.records = records;
+  a.H = num_heads;
+  a.D = head_dim;
+  a.bs = block_size;
+  a.M = max_prefix_blocks;
+  a.P = num_blocks;
+  a.scale = scale;
+  e = q_dtype == TLALOC_B200_F32 ? LaunchTiledByPool<float>(a, kv_dtype, st) : LaunchTiledByPool<__nv_bfloat16>(a, kv_dtype, st);
+  if (e != cudaSuccess) return CudaFail("SHARED_PREFIX_ATTENTION launch", e);
+  m.plan = a.plan;
+  m.prefix = records;
+  m.own = own;
+  m.lens = seq_lens;
+  m.out = out;
+  m.lse = lse;
+  m.H = num_heads;
+  m.D = head_dim;
+  m.max_own = max_blocks_per_seq * block_size;
+  const unsigned blocks = static_cast<unsigned>((static_cast<long long>(num_rows) * num_heads + kMergeWarps - 1) / kMergeWarps);
+  e = out_dtype == TLALOC_B200_F32 ? LaunchChained(PrefixMerge<float>, blocks, 32 * kMergeWarps, 0, st, m)
+                                   : LaunchChained(PrefixMerge<__nv_bfloat16>, blocks, 32 * kMergeWarps, 0, st, m);
+  if (e != cudaSuccess) return CudaFail("SHARED_PREFIX_ATTENTION merge launch", e);
+  CountLaunches(2);
+  return kOk;
+}

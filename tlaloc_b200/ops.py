@@ -56,6 +56,25 @@ def _stream(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(device)  # looked up here: a torch without CUDA does not have it, and imports this module
 
 
+def _together(op: str, like: torch.Tensor, *ts) -> None:
+    """Operands of one call: contiguous, on the device of `like`."""
+    device = like.get_device()
+    for t in ts:
+        if t is not None and (not t.is_cuda or t.get_device() != device or not t.is_contiguous()):
+            raise ValueError(f"{op}: operands must be contiguous CUDA tensors on {like.device} (there is no CPU path)")
+
+
+def _launch(like: torch.Tensor, function, *args) -> None:
+    """function(*args, stream) on the current stream of the device of `like`, with that device current."""
+    stream = _stream(like)
+    device = like.get_device()
+    if device == torch._C._cuda_getDevice():
+        N.check(function(*args, stream))
+    else:
+        with torch.cuda.device(device):
+            N.check(function(*args, stream))
+
+
 def init() -> None:
     """Kernel set-up for the current CUDA device (call once per device, before any graph capture)."""
     N.check(N.lib().tlaloc_b200_init())
@@ -100,6 +119,49 @@ def paged_attention(query, key_cache, value_cache, block_tables, seq_lens, *, sc
         _ptr(seq_lens), _ptr(keep), 0 if keep is None else keep.shape[1], _ptr(out), _dt(out), _ptr(lse),
         _ptr(scratch), scratch.shape[0], p.num_seqs, p.num_heads, p.head_dim, p.num_blocks, p.block_size,
         p.num_kv_heads, p.max_blocks_per_seq, p.num_tables, float(scale), int(sliding_window or 0), _stream(query)))
+    return (out, lse) if return_lse else out
+
+
+def shared_prefix_scratch(query, key_cache, prefix_tables, block_tables) -> torch.Tensor:
+    """The workspace of `shared_prefix_attention` for operands of these shapes."""
+    R, H, D = query.shape
+    n = N.lib().tlaloc_b200_shared_prefix_scratch_bytes(R, H, key_cache.shape[2], D, prefix_tables.shape[0], block_tables.shape[1], key_cache.shape[1])
+    return torch.empty((n // 4,), dtype=torch.float32, device=query.device)
+
+
+def shared_prefix_attention(query, key_cache, value_cache, prefix_tables, prefix_lens, row_starts, block_tables, seq_lens, *, scale, out=None, out_dtype=None,
+                            scratch=None, return_lse=False):
+    """Paged attention of rows [R, H, D] that share prefixes: row r of [row_starts[g], row_starts[g + 1]) attends the first prefix_lens[g] positions of
+    prefix_tables[g] and then its own seq_lens[r] positions of block_tables (one table per row, or per equal group of consecutive rows).  Each prefix is read once
+    for all of its rows.  See include/tlaloc_b200.h."""
+    op = "SHARED_PREFIX_ATTENTION"
+    if query.dim() != 3 or key_cache.dim() != 4 or value_cache.shape != key_cache.shape or key_cache.shape[3] != query.shape[2]:
+        raise ValueError(f"{op}: query [R, H, D] and pools [P, bs, Hkv, D] are needed, got {tuple(query.shape)}, {tuple(key_cache.shape)}, {tuple(value_cache.shape)}")
+    if prefix_tables.dim() != 2 or block_tables.dim() != 2 or prefix_lens.dim() != 1 or row_starts.dim() != 1 or seq_lens.dim() != 1:
+        raise ValueError(f"{op}: prefix_tables [G, blocks], prefix_lens [G], row_starts [G + 1], block_tables [Tb, blocks] and seq_lens [R] are needed")
+    R, H, D = query.shape
+    P, bs, Hkv, _ = key_cache.shape
+    G, Mp = prefix_tables.shape
+    if prefix_lens.shape[0] != G or row_starts.shape[0] != G + 1 or seq_lens.shape[0] != R:
+        raise ValueError(f"{op}: {G} prefixes have as many lengths and one more row start, {R} rows as many lengths; got {prefix_lens.shape[0]}, {row_starts.shape[0]}, "
+                         f"{seq_lens.shape[0]}")
+    if value_cache.dtype != key_cache.dtype:
+        raise TypeError(f"{op}: the pools have one type, got {key_cache.dtype} and {value_cache.dtype}")
+    for t in (prefix_tables, prefix_lens, row_starts, block_tables, seq_lens):
+        if t.dtype != torch.int32:
+            raise TypeError(f"{op}: tables, lengths and row starts are int32")
+    _together(op, query, query, key_cache, value_cache, prefix_tables, prefix_lens, row_starts, block_tables, seq_lens)
+    if out is None:
+        out = torch.empty((R, H, D), dtype=query.dtype if out_dtype is None else out_dtype, device=query.device)
+    _out(f"{op} out", out, (R, H, D), (torch.float32, torch.bfloat16), query)
+    if scratch is None:
+        scratch = shared_prefix_scratch(query, key_cache, prefix_tables, block_tables)
+    else:
+        _out(f"{op} scratch", scratch, None, torch.float32, query)
+    lse = torch.empty((R, H), dtype=torch.float32, device=query.device) if return_lse else None
+    _launch(query, N.lib().tlaloc_b200_shared_prefix_attention, query.data_ptr(), _dt(query), key_cache.data_ptr(), value_cache.data_ptr(), _dt(key_cache),
+            prefix_tables.data_ptr(), prefix_lens.data_ptr(), row_starts.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), _dt(out), _ptr(lse),
+            scratch.data_ptr(), scratch.numel() * 4, R, H, D, P, bs, Hkv, G, Mp, block_tables.shape[1], block_tables.shape[0], float(scale))
     return (out, lse) if return_lse else out
 
 
@@ -232,6 +294,46 @@ def rope_kv_write(q, k, v, positions, cos_table, sin_table, slot_mapping, key_ca
     return q_out
 
 
+def norm_rope_kv_write(q, k, v, positions, cos, sin, slot_mapping, key_cache, value_cache, *, q_gain=None, k_gain=None, eps=1e-6, interleaved=False, q_out=None,
+                       q_dtype=torch.bfloat16):
+    """q [T, H, hd] and k [T, Hkv, hd] normed per head (q_gain, k_gain f32 [hd], or neither) and rotated in their first 2 * cos.shape[1] channels, k and v into the pools
+    at slot_mapping; returns the queries.  q, k, v: f32 or bf16, rows of dense heads that may be column blocks of one projection; cos, sin f32 [positions, pairs]
+    (rotary.pair_tables); pairs are (i, i + pairs), or (2i, 2i + 1) with `interleaved`.  See include/tlaloc_b200.h."""
+    op = "NORM_ROPE_KV_WRITE"
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or key_cache.dim() != 4 or value_cache.shape != key_cache.shape:
+        raise ValueError(f"{op}: q [T, H, hd], k and v [T, Hkv, hd] and pools [P, bs, Hkv, hd] are needed")
+    T, H, hd = q.shape
+    Hkv = k.shape[1]
+    P, bs = key_cache.shape[:2]
+    if k.shape[0] != T or k.shape[2] != hd or key_cache.shape[2] != Hkv or key_cache.shape[3] != hd:
+        raise ValueError(f"{op}: q {tuple(q.shape)}, k and v {tuple(k.shape)}, pools {tuple(key_cache.shape)} do not fit")
+    lds = []
+    for t, heads in ((q, H), (k, Hkv), (v, Hkv)):
+        row, head, one = t.stride()
+        if not t.is_cuda or t.get_device() != q.get_device() or (one != 1 and hd > 1) or (head != hd and heads > 1):
+            raise ValueError(f"{op}: q, k and v must be CUDA tensors on {q.device} with dense heads")
+        lds.append(row if T > 1 else max(row, heads * hd))
+    if k.dtype != q.dtype or v.dtype != q.dtype or key_cache.dtype != value_cache.dtype:
+        raise TypeError(f"{op}: q, k and v have one type, and so have the pools")
+    if positions.dtype != torch.int32 or slot_mapping.dtype != torch.int32 or tuple(positions.shape) != (T,) or tuple(slot_mapping.shape) != (T,):
+        raise ValueError(f"{op}: positions and slot_mapping are int32 [{T}]")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape[0] < 1:
+        raise ValueError(f"{op}: cos and sin are f32 [positions, pairs]")
+    for g in (q_gain, k_gain):
+        if g is not None and (g.dtype != torch.float32 or tuple(g.shape) != (hd,)):
+            raise ValueError(f"{op}: gains are f32 [{hd}]")
+    _together(op, q, positions, cos, sin, slot_mapping, key_cache, value_cache, q_gain, k_gain)
+    if q_out is None:
+        q_out = torch.empty((T, H, hd), dtype=q_dtype, device=q.device)
+    _out(f"{op} q_out", q_out, (T, H, hd), (torch.float32, torch.bfloat16), q)
+    if T == 0:
+        return q_out
+    _launch(q, N.lib().tlaloc_b200_norm_rope_kv_write, q.data_ptr(), lds[0], k.data_ptr(), lds[1], v.data_ptr(), lds[2], _dt(q), _ptr(q_gain), _ptr(k_gain), float(eps),
+            positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), slot_mapping.data_ptr(), q_out.data_ptr(), _dt(q_out), key_cache.data_ptr(), value_cache.data_ptr(),
+            _dt(key_cache), T, H, Hkv, hd, 2 * cos.shape[1], int(interleaved), P * bs, cos.shape[0])
+    return q_out
+
+
 def swiglu(gate, up, *, out=None, out_dtype=torch.float32):
     """silu(gate) * up; gate and up may be column slices of one [rows, ld] matrix (a fused gate|up projection)."""
     if not gate.is_cuda or gate.stride(1) != 1 or up.stride(1) != 1 or gate.stride(0) != up.stride(0):
@@ -251,6 +353,37 @@ def argmax(logits, out=None):
         out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
     _out("ARGMAX out", out, (rows,), torch.int32, logits)
     N.check(N.lib().tlaloc_b200_argmax(_ptr(logits), _ptr(out), rows, n, _stream(logits)))
+    return out
+
+
+def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+    """One token drawn from each row of logits [rows, n] (f32 or bf16, dense rows) by the random numbers uniforms f32 [rows] in [0, 1): i32 [rows].  Each setting is a
+    number for all rows or a tensor of one per row (f32; top_k i32).  A temperature that is not above 0 is greedy; top_k 0, top_p 1 and min_p 0 keep everything.  See
+    include/tlaloc_b200.h."""
+    op = "SAMPLE"
+    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError(f"{op}: logits [rows, n] with dense rows are needed, got {tuple(logits.shape)}")
+    rows, n = logits.shape
+    if uniforms.dtype != torch.float32 or tuple(uniforms.shape) != (rows,):
+        raise ValueError(f"{op}: uniforms are f32 [{rows}], got {uniforms.dtype} {tuple(uniforms.shape)}")
+    each, every = [], []
+    for name, setting, kind in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if isinstance(setting, torch.Tensor):
+            if setting.dtype != kind or tuple(setting.shape) != (rows,):
+                raise ValueError(f"{op}: {name} of each row is {kind} [{rows}], got {setting.dtype} {tuple(setting.shape)}")
+            each.append(setting)
+            every.append(0)
+        else:
+            each.append(None)
+            every.append(max(-1, min(int(setting), 2**31 - 1)) if kind == torch.int32 else float(setting))
+    _together(op, logits, uniforms, *each)
+    if out is None:
+        out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
+    _out(f"{op} out", out, (rows,), torch.int32, logits)
+    if rows == 0:
+        return out
+    _launch(logits, N.lib().tlaloc_b200_sample, logits.data_ptr(), logits.stride(0) if rows > 1 else n, _dt(logits), uniforms.data_ptr(), *map(_ptr, each), *every,
+            out.data_ptr(), rows, n)
     return out
 
 
