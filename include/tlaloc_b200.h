@@ -163,7 +163,7 @@ int tlaloc_b200_paged_attention_static(const void* query, int32_t q_dtype, const
  *   prefix_tables  device i32 [G, max_prefix_blocks], prefix_lens device i32 [G] (0: none of it; clamped into the table)
  *   row_starts     device i32 [G + 1], not falling: prefix g is that of rows [row_starts[g], row_starts[g + 1]); rows outside have no prefix
  *   block_tables, seq_lens   the own positions of each row, as in tlaloc_b200_paged_attention (seq_lens does not count the prefix; 0: none)
- *   scratch        device memory, 16-byte aligned, contents undefined on entry and exit: tlaloc_b200_shared_prefix_scratch_bytes(...)
+ *   scratch        device memory, 32-byte aligned, contents undefined on entry and exit: tlaloc_b200_shared_prefix_scratch_bytes(...)
  * query, pools, out, lse (of all the row's keys), dtypes, scale and clamping as in tlaloc_b200_paged_attention.  A row without any key gives zeros (and lse -inf).
  * Results carry f32 accuracy where out is F32; for a BF16 out the weights of the prefix's keys may be rounded to bf16 in front of the product with the values.
  * Refused in parity mode.

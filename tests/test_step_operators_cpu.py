@@ -171,7 +171,7 @@ def c_prefix(**change):
     (dict(q=None), N.INVALID_ARGUMENT), (dict(prefix_lens=None), N.INVALID_ARGUMENT), (dict(row_starts=None), N.INVALID_ARGUMENT), (dict(lens=None), N.INVALID_ARGUMENT),
     (dict(scratch=None), N.INVALID_ARGUMENT), (dict(q_dtype=N.S8), N.INVALID_ARGUMENT), (dict(kv_dtype=N.S8), N.INVALID_ARGUMENT), (dict(out_dtype=N.F8E4M3FN), N.INVALID_ARGUMENT),
     (dict(G=0), N.INVALID_ARGUMENT), (dict(Mp=0), N.INVALID_ARGUMENT), (dict(bs=0), N.INVALID_ARGUMENT), (dict(Mp=1 << 29), N.UNSUPPORTED), (dict(scratch_bytes=64), N.INVALID_ARGUMENT),
-    (dict(scratch=at(9) + 4), N.INVALID_ARGUMENT), (dict(R=0), N.INVALID_ARGUMENT), (dict(H=5), N.INVALID_ARGUMENT), (dict(D=257), N.UNSUPPORTED), (dict(Tb=3), N.INVALID_ARGUMENT),
+    (dict(scratch=at(9) + 16), N.INVALID_ARGUMENT), (dict(R=0), N.INVALID_ARGUMENT), (dict(Hkv=0), N.INVALID_ARGUMENT), (dict(H=5), N.INVALID_ARGUMENT), (dict(D=257), N.UNSUPPORTED), (dict(Tb=3), N.INVALID_ARGUMENT),
     (dict(M=0), N.INVALID_ARGUMENT), (dict(scale=float("nan")), N.INVALID_ARGUMENT), (dict(scale=float("inf")), N.INVALID_ARGUMENT)])
 def test_c_shared_prefix_refuses(change, status):
     assert c_prefix(**change) == status

@@ -14,17 +14,6 @@
 namespace tlaloc_b200 {
 namespace {
 
-struct PrefixArgs {
-  PrefixPlan plan;
-  const void* q;
-  const void* kc;
-  const void* vc;
-  const int* tables;  // [G, M]
-  float* records;     // [max_blocks, unit_rows, D + 2]
-  int H, D, bs, M, P;
-  float scale;
-};
-
 // ------------------------------------------------------------------------------------------
 // Any type, head size and page size: f32 FMAs over tiles of 64 pairs x 32 keys in shared memory.
 
@@ -161,15 +150,15 @@ __global__ void __launch_bounds__(kTiledThreads) PrefixTiled(const __grid_consta
     for (int i = 0; i < 4; ++i) {
       const int r = ty * 4 + i;
       if (r >= s.pairs) continue;
-      float* rec = a.records + (static_cast<size_t>(s.block) * kPairs + r) * (D + 2);
+      const size_t at_r = static_cast<size_t>(s.block) * kPairs + r;
       if (tx == 0) {
-        rec[0] = m_s[r];
-        rec[1] = l_s[r];
+        a.heads[2 * at_r] = RecordMax(m_s[r], l_s[r]);
+        a.heads[2 * at_r + 1] = l_s[r];
       }
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const int d = tx + 16 * j;
-        if (d < D) rec[2 + d] = acc[i][j];
+        if (d < D) a.acc[at_r * a.d8 + d] = acc[i][j];
       }
     }
   }
@@ -180,12 +169,13 @@ __global__ void __launch_bounds__(kTiledThreads) PrefixTiled(const __grid_consta
 
 struct MergeArgs {
   PrefixPlan plan;
-  const float* prefix;  // [max_blocks, unit_rows, D + 2]
+  const float* acc;     // records of the prefixes, as in PrefixArgs
+  const float* heads;
   const float* own;     // [slices, R, H, D + 2]
   const int* lens;      // [R], own positions
   void* out;
   float* lse;
-  int H, D, max_own, slice, slices;
+  int H, D, d8, max_own, slice, slices;
 };
 
 constexpr int kMergeWarps = 4;
@@ -204,36 +194,38 @@ __global__ void __launch_bounds__(32 * kMergeWarps) PrefixMerge(const __grid_con
   const long long run = PrefixRun(a.plan, &total);
   PrefixGroup g;
   int index, shared = 0;
-  const float* first = nullptr;
-  const size_t step = static_cast<size_t>(a.plan.unit_rows) * (a.D + 2), own_step = static_cast<size_t>(a.plan.R) * a.H * (a.D + 2);
+  size_t first = 0;
+  const size_t own_step = static_cast<size_t>(a.plan.R) * a.H * (a.D + 2);
   if (PrefixFind(a.plan, true, row, &g, &index) && g.tiles > 0) {
     const int pair = (row - g.row0) * a.plan.group + head % a.plan.group;
     const long long unit = static_cast<long long>(kv) * g.units + pair / a.plan.unit_rows, work = g.work0 + unit * g.tiles;
     const long long c0 = work / run, c1 = (work + g.tiles - 1) / run, block = c0 + g.unit0 + unit;
     if (block + (c1 - c0) < a.plan.max_blocks) {
       shared = static_cast<int>(c1 - c0 + 1);
-      first = a.prefix + block * step + static_cast<size_t>(pair % a.plan.unit_rows) * (a.D + 2);
+      first = static_cast<size_t>(block) * a.plan.unit_rows + pair % a.plan.unit_rows;
     }
   }
   const float* mine = a.own + static_cast<size_t>(rh) * (a.D + 2);
   const int n = shared + own;
-  auto record = [&](int i) { return i < shared ? first + i * step : mine + (i - shared) * own_step; };
+  auto header = [&](int i) { return i < shared ? a.heads + 2 * (first + static_cast<size_t>(i) * a.plan.unit_rows) : mine + (i - shared) * own_step; };
+  auto values = [&](int i) { return i < shared ? a.acc + (first + static_cast<size_t>(i) * a.plan.unit_rows) * a.d8 : mine + (i - shared) * own_step + 2; };
   float top = -INFINITY;
-  for (int i = lane; i < n; i += 32) top = fmaxf(top, record(i)[0]);
+  for (int i = lane; i < n; i += 32) top = fmaxf(top, header(i)[0]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   float sum = 0.f, acc[8] = {};
   for (int i = 0; i < n; ++i) {
-    const float* r = record(i);
-    const float w = r[0] == -INFINITY ? 0.f : expf(r[0] - top);
+    const float* h = header(i);
+    const float w = h[0] == -INFINITY ? 0.f : expf(h[0] - top);
     if (w == 0.f) continue;
-    sum += w * r[1];
+    sum += w * h[1];
+    const float* v = values(i);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (lane + 32 * j < a.D) acc[j] += w * r[2 + lane + 32 * j];
+      if (lane + 32 * j < a.D) acc[j] += w * v[lane + 32 * j];
   }
   OT* out = static_cast<OT*>(a.out) + rh * a.D;
-  const bool empty = top == -INFINITY || sum == 0.f;
+  const bool empty = sum == 0.f;  // no keys, or none that weighs anything
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     if (lane + 32 * j < a.D) out[lane + 32 * j] = FromF32<OT>(empty ? 0.f : acc[j] / sum);
@@ -295,7 +287,10 @@ long long RecordBlocks(int rows, int heads, int kv_heads, int prefixes, int unit
   const long long pairs = static_cast<long long>(rows) * (heads / kv_heads);
   return grid + kv_heads * (pairs / unit_rows + std::min<long long>(prefixes, rows));
 }
-size_t RecordBytes(long long blocks, int unit_rows, int head_dim) { return static_cast<size_t>(blocks) * unit_rows * (head_dim + 2) * sizeof(float); }
+size_t RecordBytes(long long blocks, int unit_rows, int head_dim)
+{
+  return static_cast<size_t>(blocks) * unit_rows * ((head_dim + 7) / 8 * 8 + 2) * sizeof(float);
+}
 int OwnSlices(int max_blocks, int block_size) { return static_cast<int>((static_cast<long long>(max_blocks) * block_size + 255) / 256); }
 
 }  // namespace
@@ -307,8 +302,10 @@ extern "C" size_t tlaloc_b200_shared_prefix_scratch_bytes(int32_t num_rows, int3
                                                           int32_t max_blocks_per_seq, int32_t block_size)
 {
   if (num_rows < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1 || num_prefixes < 1 || max_blocks_per_seq < 1 || block_size < 1) return 0;
-  const size_t records = RecordBytes(RecordBlocks(num_rows, num_heads, num_kv_heads, num_prefixes, kPairs, kTiledGrid), kPairs, head_dim);
-  return records + tlaloc_b200_paged_attention_scratch_bytes(num_rows, num_heads, head_dim, OwnSlices(max_blocks_per_seq, block_size));
+  // Whichever record kernel takes the call: that hangs on types and addresses too.
+  const size_t tiled = RecordBytes(RecordBlocks(num_rows, num_heads, num_kv_heads, num_prefixes, kPairs, kTiledGrid), kPairs, head_dim);
+  const size_t tc = head_dim <= 128 ? RecordBytes(RecordBlocks(num_rows, num_heads, num_kv_heads, num_prefixes, kPrefixTcPairs, kPrefixTcGrid), kPrefixTcPairs, head_dim) : 0;
+  return std::max(tiled, tc) + tlaloc_b200_paged_attention_scratch_bytes(num_rows, num_heads, head_dim, OwnSlices(max_blocks_per_seq, block_size));
 }
 
 extern "C" int tlaloc_b200_shared_prefix_attention(const void* query, int32_t q_dtype, const void* key_cache, const void* value_cache, int32_t kv_dtype,
@@ -322,23 +319,15 @@ extern "C" int tlaloc_b200_shared_prefix_attention(const void* query, int32_t q_
   if (!prefix_tables || !prefix_lens || !row_starts || !out || !scratch) return Fail(kInvalid, "%s: a required device pointer is null", op);
   if (!IsFloatType(out_dtype)) return Fail(kInvalid, "%s: out must be f32 or bf16", op);
   if (num_prefixes < 1 || max_prefix_blocks < 1 || block_size < 1) return Fail(kInvalid, "%s: needs one prefix table or more, of one block or more", op);
+  if (num_rows < 1 || num_heads < 1 || num_kv_heads < 1 || head_dim < 1 || max_blocks_per_seq < 1) return Fail(kInvalid, "%s: needs rows, heads, channels and own blocks", op);
   if (static_cast<int64_t>(max_prefix_blocks) * block_size > (1 << 30)) return Fail(kUnsupported, "%s: a prefix of %lld positions is too long", op, static_cast<long long>(max_prefix_blocks) * block_size);
   if (OrderFaithful()) return Fail(kUnsupported, "%s: has no parity mode", op);
   const size_t need = tlaloc_b200_shared_prefix_scratch_bytes(num_rows, num_heads, num_kv_heads, head_dim, num_prefixes, max_blocks_per_seq, block_size);
-  if (scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15) != 0) {
-    return Fail(kInvalid, "%s: scratch must be 16-byte aligned and hold %zu bytes (got %zu)", op, need, scratch_bytes);
+  if (scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 31) != 0) {
+    return Fail(kInvalid, "%s: scratch must be 32-byte aligned and hold %zu bytes (got %zu)", op, need, scratch_bytes);
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int own_slices = OwnSlices(max_blocks_per_seq, block_size);
-  float* own = static_cast<float*>(scratch);
-  float* records = own + tlaloc_b200_paged_attention_scratch_bytes(num_rows, num_heads, head_dim, own_slices) / sizeof(float);
-  MergeArgs m = {};
-  // The own part first: its checks are those of all the operands that both parts share.
-  int rc = LaunchPagedSlices(op, query, q_dtype, key_cache, value_cache, kv_dtype, block_tables, seq_lens, own, own_slices, num_rows, num_heads, head_dim,
-                             num_blocks, block_size, num_kv_heads, max_blocks_per_seq, num_tables, scale, st, &m.slice, &m.slices);
-  if (rc != kOk) return rc;
-  cudaError_t e = PrepareSharedPrefix();
-  if (e != cudaSuccess) return CudaFail("SHARED_PREFIX_ATTENTION set-up", e);
   PrefixArgs a = {};
   a.plan.lens = prefix_lens;
   a.plan.starts = row_starts;
@@ -347,32 +336,47 @@ extern "C" int tlaloc_b200_shared_prefix_attention(const void* query, int32_t q_
   a.plan.group = num_heads / num_kv_heads;
   a.plan.Hkv = num_kv_heads;
   a.plan.max_len = max_prefix_blocks * block_size;
-  a.plan.unit_rows = kPairs;
-  a.plan.tile = kTileKeys;
-  a.plan.grid = kTiledGrid;
-  a.plan.min_run = 4;
-  a.plan.max_blocks = static_cast<int>(RecordBlocks(num_rows, num_heads, num_kv_heads, num_prefixes, kPairs, kTiledGrid));
   a.q = query;
   a.kc = key_cache;
   a.vc = value_cache;
   a.tables = prefix_tables;
-  a.records = records;
   a.H = num_heads;
   a.D = head_dim;
+  a.d8 = (head_dim + 7) / 8 * 8;
   a.bs = block_size;
   a.M = max_prefix_blocks;
   a.P = num_blocks;
   a.scale = scale;
-  e = q_dtype == TLALOC_B200_F32 ? LaunchTiledByPool<float>(a, kv_dtype, st) : LaunchTiledByPool<__nv_bfloat16>(a, kv_dtype, st);
+  const bool tc = PrefixTcApplies(a, q_dtype, kv_dtype);
+  a.plan.unit_rows = tc ? kPrefixTcPairs : kPairs;
+  a.plan.tile = tc ? kPrefixTcKeys : kTileKeys;
+  a.plan.grid = tc ? kPrefixTcGrid : kTiledGrid;
+  a.plan.min_run = tc ? 1 : 4;
+  a.plan.max_blocks = static_cast<int>(RecordBlocks(num_rows, num_heads, num_kv_heads, num_prefixes, a.plan.unit_rows, a.plan.grid));
+  a.acc = static_cast<float*>(scratch);
+  a.heads = a.acc + static_cast<size_t>(a.plan.max_blocks) * a.plan.unit_rows * a.d8;
+  float* own = a.heads + static_cast<size_t>(a.plan.max_blocks) * a.plan.unit_rows * 2;
+  MergeArgs m = {};
+  // The own part first: its checks are those of all the operands that both parts share.
+  int rc = LaunchPagedSlices(op, query, q_dtype, key_cache, value_cache, kv_dtype, block_tables, seq_lens, own, own_slices, num_rows, num_heads, head_dim,
+                             num_blocks, block_size, num_kv_heads, max_blocks_per_seq, num_tables, scale, st, &m.slice, &m.slices);
+  if (rc != kOk) return rc;
+  cudaError_t e = PrepareSharedPrefix();
+  if (e != cudaSuccess) return CudaFail("SHARED_PREFIX_ATTENTION set-up", e);
+  e = tc                           ? LaunchPrefixTc(a, q_dtype, kv_dtype, out_dtype, st)
+      : q_dtype == TLALOC_B200_F32 ? LaunchTiledByPool<float>(a, kv_dtype, st)
+                                   : LaunchTiledByPool<__nv_bfloat16>(a, kv_dtype, st);
   if (e != cudaSuccess) return CudaFail("SHARED_PREFIX_ATTENTION launch", e);
   m.plan = a.plan;
-  m.prefix = records;
+  m.acc = a.acc;
+  m.heads = a.heads;
   m.own = own;
   m.lens = seq_lens;
   m.out = out;
   m.lse = lse;
   m.H = num_heads;
   m.D = head_dim;
+  m.d8 = a.d8;
   m.max_own = max_blocks_per_seq * block_size;
   const unsigned blocks = static_cast<unsigned>((static_cast<long long>(num_rows) * num_heads + kMergeWarps - 1) / kMergeWarps);
   e = out_dtype == TLALOC_B200_F32 ? LaunchChained(PrefixMerge<float>, blocks, 32 * kMergeWarps, 0, st, m)

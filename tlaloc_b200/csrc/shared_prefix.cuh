@@ -128,4 +128,24 @@ __device__ __forceinline__ bool PrefixNext(const PrefixPlan& p, long long run, l
   return true;
 }
 
+// The maximum as a record has it.  Where the sum is not a number the maximum is none either: of scores that are all NaN it would be -infinity, which says "no keys".
+__device__ __forceinline__ float RecordMax(float top, float sum) { return sum != sum ? sum : top; }
+
+struct PrefixArgs {
+  PrefixPlan plan;
+  const void* q;
+  const void* kc;
+  const void* vc;
+  const int* tables;  // [G, M]
+  float* acc;         // [max_blocks, unit_rows, d8]: weighted sums of values, rows of whole 32-byte words
+  float* heads;       // [max_blocks, unit_rows, 2]: {max, sum}, the maximum in units of the natural exponential
+  int H, D, d8, bs, M, P;
+  float scale;
+};
+
+// The record kernel on the tensor cores (shared_prefix_tc.cu): what its units and tiles are, whether it takes a call, its launch.
+constexpr int kPrefixTcPairs = 256, kPrefixTcKeys = 128, kPrefixTcGrid = 148;
+bool PrefixTcApplies(const PrefixArgs& a, int q_dtype, int kv_dtype);
+cudaError_t LaunchPrefixTc(const PrefixArgs& a, int q_dtype, int kv_dtype, int out_dtype, cudaStream_t st);
+
 }  // namespace tlaloc_b200
