@@ -38,17 +38,14 @@ __global__ void __launch_bounds__(kTiledThreads) PrefixTiled(const __grid_consta
   const QT* q = static_cast<const QT*>(a.q);
   const KVT* kc = static_cast<const KVT*>(a.kc);
   const KVT* vc = static_cast<const KVT*>(a.vc);
-  long long total, run = 0, at = 0, end = 0;
-  if (warp == 0) {
-    run = PrefixRun(a.plan, &total);
-    at = blockIdx.x * run;
-    end = min(at + run, total);
-  }
+  PrefixLine line(a.plan);
+  int at = blockIdx.x * line.run;
+  const int end = min(at + line.run, line.total);
   for (;;) {
     __syncthreads();
     if (warp == 0) {
       PrefixSegment s;
-      const bool more = PrefixNext(a.plan, run, end, &at, &s);
+      const bool more = line.Next(end, &at, &s);
       if (lane == 0) {
         more_s = more ? 1 : 0;
         if (more) seg_s = s;
@@ -190,18 +187,17 @@ __global__ void __launch_bounds__(32 * kMergeWarps) PrefixMerge(const __grid_con
   if (rh >= static_cast<long long>(a.plan.R) * a.H) return;
   const int row = static_cast<int>(rh / a.H), head = static_cast<int>(rh % a.H), kv = head / a.plan.group;
   const int own = min((min(max(__ldg(a.lens + row), 0), a.max_own) + a.slice - 1) / a.slice, a.slices);
-  long long total;
-  const long long run = PrefixRun(a.plan, &total);
+  PrefixLine line(a.plan);
   PrefixGroup g;
   int index, shared = 0;
   size_t first = 0;
   const size_t own_step = static_cast<size_t>(a.plan.R) * a.H * (a.D + 2);
-  if (PrefixFind(a.plan, true, row, &g, &index) && g.tiles > 0) {
+  if (line.Find(true, row, &g, &index) && g.tiles > 0) {
     const int pair = (row - g.row0) * a.plan.group + head % a.plan.group;
-    const long long unit = static_cast<long long>(kv) * g.units + pair / a.plan.unit_rows, work = g.work0 + unit * g.tiles;
-    const long long c0 = work / run, c1 = (work + g.tiles - 1) / run, block = c0 + g.unit0 + unit;
-    if (block + (c1 - c0) < a.plan.max_blocks) {
-      shared = static_cast<int>(c1 - c0 + 1);
+    const int unit = kv * g.units + pair / a.plan.unit_rows, work = g.work0 + unit * g.tiles;
+    const int c0 = work / line.run, c1 = (work + g.tiles - 1) / line.run, block = c0 + g.unit0 + unit;
+    if (block >= 0 && block + (c1 - c0) < a.plan.max_blocks) {
+      shared = c1 - c0 + 1;
       first = static_cast<size_t>(block) * a.plan.unit_rows + pair % a.plan.unit_rows;
     }
   }
@@ -291,6 +287,11 @@ size_t RecordBytes(long long blocks, int unit_rows, int head_dim)
 {
   return static_cast<size_t>(blocks) * unit_rows * ((head_dim + 7) / 8 * 8 + 2) * sizeof(float);
 }
+// Tiles of the line at most (the device's arithmetic has 32 bits).
+long long LineTiles(int rows, int heads, int kv_heads, int prefixes, int unit_rows, int tile, long long max_len)
+{
+  return (RecordBlocks(rows, heads, kv_heads, prefixes, unit_rows, 0) + 1) * ((max_len + tile - 1) / tile);
+}
 int OwnSlices(int max_blocks, int block_size) { return static_cast<int>((static_cast<long long>(max_blocks) * block_size + 255) / 256); }
 
 }  // namespace
@@ -352,6 +353,9 @@ extern "C" int tlaloc_b200_shared_prefix_attention(const void* query, int32_t q_
   a.plan.tile = tc ? kPrefixTcKeys : kTileKeys;
   a.plan.grid = tc ? kPrefixTcGrid : kTiledGrid;
   a.plan.min_run = tc ? 1 : 4;
+  if (LineTiles(num_rows, num_heads, num_kv_heads, num_prefixes, a.plan.unit_rows, a.plan.tile, a.plan.max_len) + 2 * kTiledGrid >= (1ll << 31)) {
+    return Fail(kUnsupported, "%s: %d rows of prefixes of up to %d positions are too much for one call", op, num_rows, a.plan.max_len);
+  }
   a.plan.max_blocks = static_cast<int>(RecordBlocks(num_rows, num_heads, num_kv_heads, num_prefixes, a.plan.unit_rows, a.plan.grid));
   a.acc = static_cast<float*>(scratch);
   a.heads = a.acc + static_cast<size_t>(a.plan.max_blocks) * a.plan.unit_rows * a.d8;

@@ -10,6 +10,7 @@
 
 namespace tlaloc_b200 {
 
+// The host keeps the line shorter than 2^31 tiles (PrefixLine in shared_prefix.cu).
 struct PrefixPlan {
   const int* lens;    // [G]
   const int* starts;  // [G + 1]
@@ -23,82 +24,8 @@ struct PrefixPlan {
 
 struct PrefixGroup {
   int row0, rows, len, units, tiles;  // units of one KV head; key tiles
-  long long unit0, work0;             // units and tiles in front of it
+  int unit0, work0;                   // units and tiles in front of it
 };
-
-__device__ __forceinline__ void PrefixGroupAt(const PrefixPlan& p, int g, PrefixGroup& r)
-{
-  r.row0 = r.rows = r.len = r.units = r.tiles = 0;
-  if (g >= p.G) return;
-  const int a = min(max(__ldcg(p.starts + g), 0), p.R), b = min(max(__ldcg(p.starts + g + 1), 0), p.R);
-  r.row0 = a;
-  r.rows = max(b - a, 0);
-  r.len = min(max(__ldcg(p.lens + g), 0), p.max_len);
-  r.units = r.len > 0 ? (r.rows * p.group + p.unit_rows - 1) / p.unit_rows : 0;
-  r.tiles = (r.len + p.tile - 1) / p.tile;
-}
-
-__device__ __forceinline__ long long WarpSum(long long v)
-{
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// Tiles of a run.  The whole warp.
-__device__ __forceinline__ long long PrefixRun(const PrefixPlan& p, long long* total)
-{
-  long long w = 0;
-  const int lane = threadIdx.x & 31;
-  for (int g = lane; g < p.G; g += 32) {
-    PrefixGroup r;
-    PrefixGroupAt(p, g, r);
-    w += static_cast<long long>(r.units) * p.Hkv * r.tiles;
-  }
-  w = WarpSum(w);
-  *total = w;
-  return max((w + p.grid - 1) / p.grid, static_cast<long long>(p.min_run));
-}
-
-// The group that holds tile `work` of the line (by_row false), or query row `row` (by_row true).  The whole warp; false if there is none.
-__device__ __forceinline__ bool PrefixFind(const PrefixPlan& p, bool by_row, long long at, PrefixGroup* found, int* index)
-{
-  const int lane = threadIdx.x & 31;
-  long long unit_base = 0, work_base = 0;
-  for (int g0 = 0; g0 < p.G; g0 += 32) {
-    PrefixGroup r;
-    PrefixGroupAt(p, g0 + lane, r);
-    const long long units = static_cast<long long>(r.units) * p.Hkv, work = units * r.tiles;
-    long long u = units, w = work;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long uu = __shfl_up_sync(0xffffffffu, u, o), ww = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) {
-        u += uu;
-        w += ww;
-      }
-    }
-    r.unit0 = unit_base + u - units;
-    r.work0 = work_base + w - work;
-    const bool here = by_row ? at >= r.row0 && at < r.row0 + r.rows : at >= r.work0 && at < r.work0 + work;
-    const unsigned any = __ballot_sync(0xffffffffu, here);
-    if (any != 0u) {
-      const int src = __ffs(any) - 1;
-      found->row0 = __shfl_sync(0xffffffffu, r.row0, src);
-      found->rows = __shfl_sync(0xffffffffu, r.rows, src);
-      found->len = __shfl_sync(0xffffffffu, r.len, src);
-      found->units = __shfl_sync(0xffffffffu, r.units, src);
-      found->tiles = __shfl_sync(0xffffffffu, r.tiles, src);
-      found->unit0 = __shfl_sync(0xffffffffu, r.unit0, src);
-      found->work0 = __shfl_sync(0xffffffffu, r.work0, src);
-      *index = g0 + src;
-      return true;
-    }
-    unit_base += __shfl_sync(0xffffffffu, u, 31);
-    work_base += __shfl_sync(0xffffffffu, w, 31);
-  }
-  return false;
-}
 
 // What one CTA does of one unit: pairs [pair0, pair0 + pairs) of the group's (row, head of the KV head) pairs, key tiles [tile0, tile1).
 struct PrefixSegment {
@@ -106,27 +33,105 @@ struct PrefixSegment {
   int block;  // of the records; -1: there is no room (row ranges that overlap one another)
 };
 
-// The segment at `at` of a run that ends at `end`; moves `at` behind it.  The whole warp.
-__device__ __forceinline__ bool PrefixNext(const PrefixPlan& p, long long run, long long end, long long* at, PrefixSegment* s)
-{
-  PrefixGroup g;
-  int index = 0;
-  if (*at >= end || !PrefixFind(p, false, *at, &g, &index)) return false;
-  const long long in = *at - g.work0;
-  const int unit = static_cast<int>(in / g.tiles);
-  s->tile0 = static_cast<int>(in % g.tiles);
-  s->tile1 = static_cast<int>(min(static_cast<long long>(g.tiles), s->tile0 + end - *at));
-  s->row0 = g.row0;
-  s->len = g.len;
-  s->index = index;
-  s->kv = unit / g.units;
-  s->pair0 = (unit % g.units) * p.unit_rows;
-  s->pairs = min(p.unit_rows, g.rows * p.group - s->pair0);
-  const long long block = *at / run + g.unit0 + unit;
-  s->block = block < p.max_blocks ? static_cast<int>(block) : -1;
-  *at += s->tile1 - s->tile0;
-  return true;
-}
+// A warp's view of the groups, 32 at a time, a lane one; the first 32 are read once.  All functions take the whole warp.
+class PrefixLine {
+ public:
+  int run, total;  // tiles of a CTA's run, and of the line
+
+  __device__ __forceinline__ explicit PrefixLine(const PrefixPlan& p) : p_(p)
+  {
+    Load(0, 0, 0);
+    total = work_end_;
+    int units = unit_end_;
+    for (int g0 = 32; g0 < p.G; g0 += 32) {
+      Load(g0, units, total);
+      total = work_end_;
+      units = unit_end_;
+    }
+    if (p.G > 32) Load(0, 0, 0);
+    run = max((total + p.grid - 1) / p.grid, p.min_run);
+  }
+
+  // The group that holds tile `at` of the line (by_row false), or query row `at` (by_row true); false if there is none.
+  __device__ __forceinline__ bool Find(bool by_row, int at, PrefixGroup* found, int* index)
+  {
+    if (g0_ != 0) Load(0, 0, 0);
+    for (;;) {
+      const bool here = by_row ? at >= mine_.row0 && at < mine_.row0 + mine_.rows : at >= mine_.work0 && at < mine_.work0 + mine_.units * p_.Hkv * mine_.tiles;
+      const unsigned any = __ballot_sync(0xffffffffu, here);
+      if (any != 0u) {
+        const int src = __ffs(any) - 1;
+        found->row0 = __shfl_sync(0xffffffffu, mine_.row0, src);
+        found->rows = __shfl_sync(0xffffffffu, mine_.rows, src);
+        found->len = __shfl_sync(0xffffffffu, mine_.len, src);
+        found->units = __shfl_sync(0xffffffffu, mine_.units, src);
+        found->tiles = __shfl_sync(0xffffffffu, mine_.tiles, src);
+        found->unit0 = __shfl_sync(0xffffffffu, mine_.unit0, src);
+        found->work0 = __shfl_sync(0xffffffffu, mine_.work0, src);
+        *index = g0_ + src;
+        return true;
+      }
+      if (g0_ + 32 >= p_.G) return false;
+      Load(g0_ + 32, unit_end_, work_end_);
+    }
+  }
+
+  // The segment at `at` of a run that ends at `end`; moves `at` behind it.
+  __device__ __forceinline__ bool Next(int end, int* at, PrefixSegment* s)
+  {
+    PrefixGroup g;
+    int index = 0;
+    if (*at >= end || !Find(false, *at, &g, &index)) return false;
+    const int in = *at - g.work0, unit = in / g.tiles;
+    s->tile0 = in - unit * g.tiles;
+    s->tile1 = min(g.tiles, s->tile0 + end - *at);
+    s->row0 = g.row0;
+    s->len = g.len;
+    s->index = index;
+    s->kv = unit / g.units;
+    s->pair0 = (unit - s->kv * g.units) * p_.unit_rows;
+    s->pairs = min(p_.unit_rows, g.rows * p_.group - s->pair0);
+    const int block = static_cast<int>(blockIdx.x) + g.unit0 + unit;
+    s->block = block >= 0 && block < p_.max_blocks ? block : -1;
+    *at += s->tile1 - s->tile0;
+    return true;
+  }
+
+ private:
+  const PrefixPlan& p_;
+  PrefixGroup mine_;  // this lane's of the groups [g0_, g0_ + 32)
+  int g0_, unit_end_, work_end_;
+
+  __device__ __forceinline__ void Load(int g0, int unit_base, int work_base)
+  {
+    const int lane = threadIdx.x & 31, g = g0 + lane;
+    PrefixGroup r = {};
+    if (g < p_.G) {
+      const int a = min(max(__ldcg(p_.starts + g), 0), p_.R), b = min(max(__ldcg(p_.starts + g + 1), 0), p_.R);
+      r.row0 = a;
+      r.rows = max(b - a, 0);
+      r.len = min(max(__ldcg(p_.lens + g), 0), p_.max_len);
+      r.units = r.len > 0 ? (r.rows * p_.group + p_.unit_rows - 1) / p_.unit_rows : 0;
+      r.tiles = (r.len + p_.tile - 1) / p_.tile;
+    }
+    const int units = r.units * p_.Hkv, work = units * r.tiles;
+    int u = units, w = work;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int uu = __shfl_up_sync(0xffffffffu, u, o), ww = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) {
+        u += uu;
+        w += ww;
+      }
+    }
+    r.unit0 = unit_base + u - units;
+    r.work0 = work_base + w - work;
+    mine_ = r;
+    g0_ = g0;
+    unit_end_ = unit_base + __shfl_sync(0xffffffffu, u, 31);
+    work_end_ = work_base + __shfl_sync(0xffffffffu, w, 31);
+  }
+};
 
 // The maximum as a record has it.  Where the sum is not a number the maximum is none either: of scores that are all NaN it would be -infinity, which says "no keys".
 __device__ __forceinline__ float RecordMax(float top, float sum) { return sum != sum ? sum : top; }

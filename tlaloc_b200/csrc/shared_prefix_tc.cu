@@ -1,13 +1,16 @@
 // Records of shared prefixes on the tensor cores: bf16 pools, head sizes of multiples of 8 up to 128, pages of multiples of 8 positions.
 //
 // The (row, head) pairs that read one KV head of a prefix are the rows of a matrix product: S = Q K^T over tiles of 128 pairs x 128 keys, O += P V, both tcgen05.mma
-// kind::f16 with f32 accumulators in TMEM, keys and values by TMA out of their pages.  A CTA runs two streams of tiles, each with its own scores, weights (in the scores'
+// kind::f16 with f32 accumulators in TMEM, keys and values by TMA out of their pages.  A CTA runs two streams, each with its own scores, weights (in the scores'
 // place), outputs and running maximum, so that one's products run under the other's softmax:
-//   a unit of more than 128 pairs    a stream takes 128 pairs and every tile of keys: a tile is fetched once for both
-//   a unit of up to 128 pairs        the streams take the same pairs and every second tile of keys, and merge their results in the end
-//   producer warp   a tile's boxes (64 channels x as many positions as lie in one page), each lane some of them, onto a ring of slots
-//   MMA lane        in turn for the streams: O += P(j) V(j), S(j + 1)
-//   eight warps     softmax, stream w by warps 4 w .. 4 w + 3, a thread a pair; before that the queries into shared memory, at the end the records
+//   a unit of more than 128 pairs    a stream takes 128 pairs and all keys: a tile of them is fetched once for both
+//   a unit of up to 128 pairs        both streams take the same pairs, one the first half of every tile of keys and one the second, and merge their results in the end
+//   three warps     tiles onto a ring of slots, in turn: a tile's boxes (64 channels x as many positions as lie in one page), each lane some of them (a warp's boxes leave
+//                   one after the other, 85 cycles each: 16 of 16 positions by one warp alone were late)
+//   MMA lane        in turn for the streams: O += P(i) V(i), S(i + 1)
+//   sixteen warps   softmax, a stream's by eight: two threads a pair, each half of its scores; before that the queries into shared memory, at the end the records
+// What bounds it where many pairs share a prefix is shared memory, which feeds both operands of S and one of O: 64-key scores in two places, which spare the softmax its
+// waits, read the queries twice as often and were no faster.
 // An f32 query enters as two bf16 parts.  Where the result is f32 the weights do as well (2^-17 of them is lost); for a bf16 result one part is enough: what is lost
 // (2^-9 of each weight, at random) is less than the result's own rounding.
 // Every mbarrier wait is bounded.
@@ -23,13 +26,16 @@ namespace {
 
 using namespace tc;
 
-constexpr int kRows = 128, kKeys = kPrefixTcKeys;
+constexpr int kRows = 128, kKeys = kPrefixTcKeys, kHalf = kKeys / 2;
 constexpr int kAtom = kRows * 64 * 2;  // 128 rows x 64 channels
-constexpr int kWarps = 8, kThreads = kWarps * 32 + 64;
+constexpr int kWarps = 16, kProducers = 3, kThreads = (kWarps + 1 + kProducers) * 32;
 constexpr int kBudget = 224 * 1024;    // queries and ring; a KB to align them and static shared memory come on top
 constexpr int kMaxSlots = 8;
 constexpr float kLazy = 8.f;           // how far (log2) a row's maximum may grow past the reference in use
 constexpr float kLn2 = 0.6931471805599453f;
+// An addition to an accumulator in TMEM drops what lies below its last place, toward zero: about 1.5e-8 of it each time (measured: 900 of them 1.4e-5).  An f32 result
+// is therefore summed over at most this many tiles (64 additions) there, and over them with rounding, in its record.
+constexpr int kChain = 4;
 
 __device__ int g_prefix_status = 0;
 
@@ -54,6 +60,32 @@ __device__ __forceinline__ uint32_t Pack(float a, float b)
   const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// Two f32 at a time.
+__device__ __forceinline__ uint64_t Both(float a, float b)
+{
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void Apart(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t Fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t Add2(uint64_t a, uint64_t b)
+{
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float Max3(float a, float b, float c)
+{
+  float r;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float Low(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float High(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 __device__ __forceinline__ void Store32(uint32_t dst, uint4 v)
@@ -68,7 +100,15 @@ __device__ __forceinline__ void StoreSector(float* dst, const float* v)
                : "memory");
 }
 __device__ __forceinline__ void FenceAsync() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
-__device__ __forceinline__ void SoftmaxWarpsSync() { asm volatile("bar.sync 1, 256;\n" ::: "memory"); }
+__device__ __forceinline__ void SoftmaxWarpsSync() { asm volatile("bar.sync 1, 512;\n" ::: "memory"); }
+// The two warps that share 32 pairs: whether any of their threads says so.
+__device__ __forceinline__ bool EitherWarp(int id, bool mine)
+{
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %2, 0;\n\tbar.red.or.pred q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n" : "=r"(r) : "r"(id), "r"(mine ? 1 : 0) : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void WarpsSync(int id) { asm volatile("bar.sync %0, 64;\n" ::"r"(id) : "memory"); }
 
 // ATOMS: 64-channel blocks of a head.  PLO: the weights in two parts.
 template <typename QT, int ATOMS>
@@ -80,10 +120,21 @@ struct PrefixTcLayout {
   static constexpr int kBytes = 2 * kQTile + kSlots * kPart + 1024;
 };
 
-// The order in which a segment's n tiles of keys (0, 2, ..) and values (1, 3, ..) are used, as places in the ring's sequence.  One stream takes tiles one after the other
-// (K0 V0 K1 V1 ..); two streams of alternate tiles want both first scores ahead (K0 K1 V0 K2 V1 ..).
-__device__ __forceinline__ int KeyItem(bool split, int t) { return !split ? 2 * t : (t == 0 ? 0 : 2 * t - 1); }
-__device__ __forceinline__ int ValueItem(bool split, int n, int t) { return !split ? 2 * t + 1 : (t == n - 1 ? 2 * n - 1 : 2 * t + 2); }
+// What the streams do in a segment: step i is tile i, all of it (up to 128 keys) or the stream's half.
+struct PrefixSteps {
+  int n, live_last;  // tiles; positions of the last one
+  bool pair_tiles;   // more than 128 pairs: each stream has pairs of its own
+  __device__ __forceinline__ explicit PrefixSteps(const PrefixSegment& s)
+      : n(s.tile1 - s.tile0), live_last(min(kKeys, s.len - (s.tile1 - 1) * kKeys)), pair_tiles(s.pairs > kRows)
+  {
+  }
+  __device__ __forceinline__ int count(int w) const { return n - (!pair_tiles && w == 1 && live_last <= kHalf ? 1 : 0); }
+  __device__ __forceinline__ int first(int w) const { return pair_tiles ? 0 : w * kHalf; }
+  __device__ __forceinline__ int live(int w, int i) const  // positions of the step, from first(w) on
+  {
+    return min(pair_tiles ? kKeys : kHalf, (i == n - 1 ? live_last : kKeys) - first(w));
+  }
+};
 
 template <typename QT, int ATOMS, bool PLO>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -94,10 +145,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ unsigned char smem_raw[];
   __shared__ alignas(8) uint64_t bars[2 * kMaxSlots + 7];
   __shared__ uint32_t slot_store[2];
+  __shared__ float s_top[2][kRows];
   const uint32_t base = (SmemAddr(smem_raw) + 1023u) & ~1023u;
   unsigned char* smem = smem_raw + (base - SmemAddr(smem_raw));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // full: a slot's tile has landed; empty: its products are done.  Per stream, sfull: scores are there; pfull: weights are; odone: the last product of a segment is done.
+  // full: a slot's tile has landed; empty: its products are done.  Per stream, sfull: scores are there (and the product before them is done); pfull: weights are; odone: the
+  // last product of a segment is done.
   const uint32_t full = SmemAddr(bars), empty = full + 8 * kMaxSlots, sfull = empty + 8 * kMaxSlots, pfull = sfull + 16, odone = pfull + 16, qfull = odone + 16;
   const uint32_t ring = base + 2 * Layout::kQTile;
   volatile uint32_t* slot = slot_store;
@@ -110,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       MbarInit(sfull + 8 * i, 1);
-      MbarInit(pfull + 8 * i, 4);
+      MbarInit(pfull + 8 * i, kWarps / 2);
       MbarInit(odone + 8 * i, 1);
     }
     MbarInit(qfull, kWarps);
@@ -126,218 +179,284 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *slot;  // S of stream w at column 128 w, O at 256 + 128 w
   GridDependencySync();
   bool ok = true;
-  long long total;
-  const long long run = PrefixRun(a.plan, &total);
-  long long at = blockIdx.x * run;
-  const long long end = min(at + run, total);
+  PrefixLine line(a.plan);
+  int at = blockIdx.x * line.run;
+  const int end = min(at + line.run, line.total);
   PrefixSegment s;
-  int items = 0;  // of the ring, in front of this segment
+  int items = 0;  // of the ring, in front of this segment: keys and values of its tiles in turn
 
-  if (warp == kWarps) {
+  if (warp > kWarps) {
     const int boxes = kKeys / box, atom = lane / boxes, mine = lane - atom * boxes;  // up to 32 boxes an item: 16 of 8 positions by two atoms
-    while (PrefixNext(a.plan, run, end, &at, &s)) {
-      const int n = s.tile1 - s.tile0;
-      const bool split = s.pairs <= kRows && n > 1;
+    int it = warp - kWarps - 1;                                                       // this warp's next item
+    while (line.Next(end, &at, &s)) {
+      const int last = items + 2 * (s.tile1 - s.tile0);
       const int* table = a.tables + static_cast<size_t>(s.index) * a.M;
-      auto tile_of = [&](int i, bool* value) {
-        if (!split) {
-          *value = (i & 1) != 0;
-          return i >> 1;
-        }
-        *value = i == 2 * n - 1 || (i > 0 && (i & 1) == 0);
-        return i == 0 ? 0 : i == 2 * n - 1 ? n - 1 : (i & 1) != 0 ? (i + 1) >> 1 : (i >> 1) - 1;
-      };
       auto row_of = [&](int i) {  // the first pool row of this lane's box, -1 if it lies past the prefix's end
-        bool value;
-        const int pos = (s.tile0 + tile_of(i, &value)) * kKeys + mine * box;
-        if (atom >= ATOMS || pos >= s.len) return -1;
+        const int pos = (s.tile0 + ((i - items) >> 1)) * kKeys + mine * box;
+        if (i >= last || atom >= ATOMS || pos >= s.len) return -1;
         const int page = min(max(__ldg(table + pos / a.bs), 0), a.P - 1);
         return page * a.bs + pos % a.bs;
       };
-      int row = row_of(0);
-      for (int i = 0; i < 2 * n; ++i) {
-        const int it = items + i, sl = it % kSlots, use = it / kSlots;
-        const int next = i + 1 < 2 * n ? row_of(i + 1) : -1;  // on its way while the slot is waited for
+      int row = row_of(it);
+      for (; it < last; it += kProducers) {
+        const int sl = it % kSlots, use = it / kSlots;
+        const int next = row_of(it + kProducers);  // on its way while the slot is waited for
         if (use > 0) ok = MbarWaitWarp(empty + 8 * sl, (use - 1) & 1, lane, abort_word) && ok;
         const unsigned live = __ballot_sync(0xffffffffu, row >= 0);
-        bool value;
-        tile_of(i, &value);
         if (lane == 0) MbarExpectTx(full + 8 * sl, __popc(live) * box * 128);
         __syncwarp();
-        if (row >= 0) TmaBox(ring + sl * kPart + atom * kAtom + mine * box * 128, value ? &map_v : &map_k, atom * 64, s.kv, row, full + 8 * sl);
+        if (row >= 0) TmaBox(ring + sl * kPart + atom * kAtom + mine * box * 128, (it & 1) != 0 ? &map_v : &map_k, atom * 64, s.kv, row, full + 8 * sl);
         row = next;
       }
-      items += 2 * n;
+      items = last;
     }
     if (!ok) {  // given up: let the copies in flight land before the CTA's shared memory goes away
       volatile uint32_t never = 0;
-      for (int it = max(0, items - kSlots); it < items; ++it) MbarWaitWarp(full + 8 * (it % kSlots), (it / kSlots) & 1, lane, &never);
+      for (int k = max(0, items - kSlots); k < items; ++k) MbarWaitWarp(full + 8 * (k % kSlots), (k / kSlots) & 1, lane, &never);
     }
-  } else if (warp == kWarps + 1) {
-    const uint32_t s_idesc = InstrDesc(kKeys, false), o_idesc = InstrDesc((a.D + 15) / 16 * 16, true);
+  } else if (warp == kWarps) {
+    // One lane issues everything, between softmax warps that want the same issue slots: what it does besides waiting and issuing is kept to a minimum.
+    const uint32_t o_idesc = InstrDesc((a.D + 15) / 16 * 16, true);
     const uint64_t qd = SmemDesc(base, 16, 1024), kd = SmemDesc(ring, 16, 1024), vd = SmemDesc(ring, kAtom, 1024);
-    const int steps = (a.D + 15) / 16;  // of 16 channels
-    int segment = 0, done[2] = {0, 0};
-    while (PrefixNext(a.plan, run, end, &at, &s)) {
-      const int n = s.tile1 - s.tile0;
-      const bool pair_tiles = s.pairs > kRows, split = !pair_tiles && n > 1;
-      const int count[2] = {pair_tiles ? n : (n + 1) / 2, pair_tiles ? n : n / 2};
+    const int depth = (a.D + 15) / 16;  // channels by 16
+    uint32_t segment = 0;
+    int done0 = 0, done1 = 0;  // steps of the streams in front of a segment
+    while (line.Next(end, &at, &s)) {
+      const PrefixSteps steps(s);
+      const bool pair_tiles = steps.pair_tiles;
+      const int count0 = steps.count(0), count1 = steps.count(1);
       if (ElectOne()) {
+        uint32_t at_slot = items % kSlots, at_phase = items / kSlots & 1;  // of the next item of the ring
         ok = MbarWait(qfull, segment & 1, abort_word) && ok;
-        auto scores = [&](int w, int j) {
-          const int t = pair_tiles ? j : 2 * j + w, it = items + KeyItem(split, t), sl = it % kSlots;
-          ok = MbarWait(full + 8 * sl, (it / kSlots) & 1, abort_word) && ok;
-          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-          // The stream's last weights lay here; their product is in front of these MMAs in the same queue.
+        auto take = [&]() {  // the next item, once it has landed: items are first used in the ring's order
+          const uint32_t sl = at_slot;
+          ok = MbarWait(full + 8 * sl, at_phase, abort_word) && ok;
+          if (++at_slot == kSlots) {
+            at_slot = 0;
+            at_phase ^= 1;
+          }
+          return sl;
+        };
+        const uint32_t s_idesc = InstrDesc(pair_tiles ? kKeys : kHalf, false);
+        auto scores = [&](int w, uint32_t sl) {
+          // The weights of the step before lay here; their product is in front of these MMAs in the same queue.
           const uint32_t acc = tmem + w * 128;
+          const uint64_t q0 = qd + static_cast<uint64_t>((pair_tiles ? w : 0) * (Layout::kQTile >> 4));
+          const uint64_t k0 = kd + static_cast<uint64_t>(sl * (kPart >> 4) + steps.first(w) * (128 >> 4));
 #pragma unroll
           for (int part = 0; part < (Layout::kQLo ? 2 : 1); ++part) {
-            const uint64_t qa = qd + static_cast<uint64_t>(((pair_tiles ? w : 0) * Layout::kQTile + part * kPart) >> 4);
-            const uint64_t ka = kd + static_cast<uint64_t>((sl * kPart) >> 4);
+            const uint64_t qa = q0 + static_cast<uint64_t>(part * (kPart >> 4));
 #pragma unroll
             for (int k = 0; k < 4 * ATOMS; ++k)
-              if (k < steps) TcMmaBf16(acc, qa + (k >> 2) * (kAtom >> 4) + 2 * (k & 3), ka + (k >> 2) * (kAtom >> 4) + 2 * (k & 3), s_idesc, part > 0 || k > 0 ? 1u : 0u);
+              if (k < depth) TcMmaBf16(acc, qa + (k >> 2) * (kAtom >> 4) + 2 * (k & 3), k0 + (k >> 2) * (kAtom >> 4) + 2 * (k & 3), s_idesc, part > 0 || k > 0 ? 1u : 0u);
           }
           TcCommit(sfull + 8 * w);
-          if (!pair_tiles || w == 1) TcCommit(empty + 8 * sl);
         };
-        scores(0, 0);
-        if (count[1] > 0) scores(1, 0);
-        for (int j = 0; j < count[0]; ++j) {
-#pragma unroll
+        uint32_t kslot = take();
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        scores(0, kslot);
+        if (count1 > 0) scores(1, kslot);
+        TcCommit(empty + 8 * kslot);
+#pragma unroll 1
+        for (int i = 0; i < count0; ++i) {
+          const uint32_t vslot = take();
+          const bool more = i + 1 < count0;
+          if (more) kslot = take();
+#pragma unroll 1
           for (int w = 0; w < 2; ++w) {
-            if (j >= count[w]) continue;
-            const int t = pair_tiles ? j : 2 * j + w, it = items + ValueItem(split, n, t), sl = it % kSlots;
-            const int live = min(kKeys, s.len - (s.tile0 + t) * kKeys);
-            ok = MbarWait(full + 8 * sl, (it / kSlots) & 1, abort_word) && ok;
-            ok = MbarWait(pfull + 8 * w, (done[w] + j) & 1, abort_word) && ok;
+            const int count = w == 0 ? count0 : count1, g = (w == 0 ? done0 : done1) + i;
+            if (i >= count) continue;
+            const int live = steps.live(w, i);
+            ok = MbarWait(pfull + 8 * w, g & 1, abort_word) && ok;
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-            // P: eight columns per 16 keys; V: keys are its rows, 16 of them per step; those that hold none are left out
+            // P: eight columns per 16 keys, a part's 16 per 32 keys together; V: keys are its rows, 16 of them per MMA; those that hold none are left out
             const uint32_t pa = tmem + w * 128, acc = tmem + 256 + w * 128;
-            const uint64_t va = vd + static_cast<uint64_t>((sl * kPart) >> 4);
+            const uint64_t va = vd + static_cast<uint64_t>(vslot * (kPart >> 4) + steps.first(w) * (128 >> 4));
+            const uint32_t add = (PLO ? i % kChain == 0 : i == 0) ? 0u : 1u;
 #pragma unroll
             for (int part = 0; part < (PLO ? 2 : 1); ++part) {
 #pragma unroll
               for (int k = 0; k < kKeys / 16; ++k)
-                if (16 * k < live) TcMmaTmemA(acc, pa + 64 * part + 8 * k, va + ((k * 16 * 128) >> 4), o_idesc, j > 0 || part > 0 || k > 0 ? 1u : 0u);
+                if (16 * k < live) TcMmaTmemA(acc, pa + 32 * (k >> 1) + 16 * part + 8 * (k & 1), va + ((k * 16 * 128) >> 4), o_idesc, part > 0 || k > 0 ? 1u : add);
             }
-            if (!pair_tiles || w == 1) TcCommit(empty + 8 * sl);
-            if (j + 1 == count[w]) TcCommit(odone + 8 * w);
-            else scores(w, j + 1);
+            if (i + 1 < count) scores(w, kslot);
+            else TcCommit(odone + 8 * w);
           }
+          TcCommit(empty + 8 * vslot);
+          if (more) TcCommit(empty + 8 * kslot);
         }
       }
       __syncwarp();
-      items += 2 * n;
-      done[0] += count[0];
-      done[1] += count[1];
+      items += 2 * steps.n;
+      done0 += count0;
+      done1 += count1;
       ++segment;
     }
   } else {
-    const int w = warp >> 2, quad = warp & 3, r = quad * 32 + lane;  // this thread's stream and TMEM lane
-    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16, sa = tmem + lanes + w * 128, oa = tmem + lanes + 256;
+    const int w = warp >> 3, h = (warp >> 2) & 1, quad = warp & 3, r = quad * 32 + lane;  // this thread's stream, half of its scores, and TMEM lane
+    const int meet = 2 + w * 4 + quad;  // the named barrier of the two warps of these pairs
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16, oa = tmem + lanes + 256;
+    constexpr int kCols = ATOMS * 32;  // of a stream's outputs that a thread sees to
     // The scale's sign (or its being zero) goes into the queries: the largest score is the largest scaled one, and no masked score is multiplied by zero.
     const float scale_log2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f, sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
-    int tiles_done = 0, segments = 0;
-    while (PrefixNext(a.plan, run, end, &at, &s)) {
-      const int n = s.tile1 - s.tile0;
-      const bool pair_tiles = s.pairs > kRows, split = !pair_tiles && n > 1;
-      const int count = pair_tiles ? n : (n + 1 - w) / 2;
+    int steps_done = 0, segments = 0;
+    while (line.Next(end, &at, &s)) {
+      const PrefixSteps steps(s);
+      const int count = steps.count(w);
       // Queries: rows of 128 bytes an atom, swizzled as TMA would; zeros for pairs and channels that are not there.
-      constexpr int kChunks = ATOMS * 8;
-      for (int i = tid; i < (pair_tiles ? 2 * kRows : kRows) * kChunks; i += kWarps * 32) {
-        const int pair = i / kChunks, c = i % kChunks;
-        float v[8] = {};
-        if (pair < s.pairs && c * 8 < a.D) {
-          const int p = s.pair0 + pair;
-          const QT* src = static_cast<const QT*>(a.q) + (static_cast<size_t>(s.row0 + p / a.plan.group) * a.H + s.kv * a.plan.group + p % a.plan.group) * a.D + c * 8;
-          if constexpr (Layout::kQLo) {
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(src)), y = __ldcg(reinterpret_cast<const float4*>(src) + 1);
-            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-          } else {
-            const uint4 x = __ldcg(reinterpret_cast<const uint4*>(src));
-            v[0] = Low(x.x), v[1] = High(x.x), v[2] = Low(x.y), v[3] = High(x.y), v[4] = Low(x.z), v[5] = High(x.z), v[6] = Low(x.w), v[7] = High(x.w);
+      constexpr int kChunks = ATOMS * 8, kPass = kWarps * 32 / kChunks;  // 16-byte words of a row; rows that the threads read at a time
+      {
+        const int c = tid % kChunks, first = tid / kChunks, n = steps.pair_tiles ? 2 * kRows : kRows;
+        constexpr int kAhead = 4;
+        for (int p0 = first; p0 < n; p0 += kAhead * kPass) {
+          uint4 raw[kAhead][Layout::kQLo ? 2 : 1];
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            const int pair = p0 + u * kPass, p = s.pair0 + pair, row = p / a.plan.group;
+            const bool there = pair < s.pairs && c * 8 < a.D;
+            const QT* src = static_cast<const QT*>(a.q) + (static_cast<size_t>(s.row0 + row) * a.H + s.kv * a.plan.group + (p - row * a.plan.group)) * a.D + c * 8;
+#pragma unroll
+            for (int e = 0; e < (Layout::kQLo ? 2 : 1); ++e) raw[u][e] = there ? __ldcg(reinterpret_cast<const uint4*>(src) + e) : make_uint4(0u, 0u, 0u, 0u);
+          }
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            const int pair = p0 + u * kPass;
+            if (pair >= n) continue;
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float x, y;
+              if constexpr (Layout::kQLo) {
+                const uint4 v = raw[u][e >> 1];
+                x = __uint_as_float((e & 1) != 0 ? v.z : v.x), y = __uint_as_float((e & 1) != 0 ? v.w : v.y);
+              } else {
+                const uint32_t v = e == 0 ? raw[u][0].x : e == 1 ? raw[u][0].y : e == 2 ? raw[u][0].z : raw[u][0].w;
+                x = Low(v), y = High(v);
+              }
+              x *= sign;
+              y *= sign;
+              hi[e] = Pack(x, y);
+              lo[e] = Pack(x - Low(hi[e]), y - High(hi[e]));
+            }
+            const uint32_t dst = base + (pair >> 7) * Layout::kQTile + (c >> 3) * kAtom + (pair & 127) * 128 + (((c & 7) ^ (pair & 7)) << 4);
+            Store32(dst, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+            if constexpr (Layout::kQLo) Store32(dst + kPart, make_uint4(lo[0], lo[1], lo[2], lo[3]));
           }
         }
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = v[2 * e] * sign, y = v[2 * e + 1] * sign;
-          hi[e] = Pack(x, y);
-          lo[e] = Pack(x - Low(hi[e]), y - High(hi[e]));
-        }
-        const uint32_t dst = base + (pair >> 7) * Layout::kQTile + (c >> 3) * kAtom + (pair & 127) * 128 + (((c & 7) ^ (pair & 7)) << 4);
-        Store32(dst, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-        if constexpr (Layout::kQLo) Store32(dst + kPart, make_uint4(lo[0], lo[1], lo[2], lo[3]));
       }
       FenceAsync();
       __syncwarp();
       if (lane == 0) MbarArrive(qfull);
-      const bool live_warp = (pair_tiles ? w * kRows : 0) + quad * 32 < s.pairs;
-      float top = -INFINITY, sum = 0.f;
-      for (int j = 0; j < count; ++j) {
-        const int t = pair_tiles ? j : 2 * j + w, live = min(kKeys, s.len - (s.tile0 + t) * kKeys);
-        ok = MbarWaitWarp(sfull + 8 * w, tiles_done & 1, lane, abort_word) && ok;
-        ++tiles_done;
+      const int own_pair = (steps.pair_tiles ? w * kRows : 0) + r;  // of the unit
+      const bool live_warp = own_pair - lane < s.pairs, mine = s.block >= 0 && own_pair < s.pairs;
+      const int chunks = steps.pair_tiles ? 2 : 1;  // of 32 scores
+      const uint32_t sa = tmem + lanes + w * 128 + h * chunks * 32, oh = oa + w * 128 + h * kCols;
+      // The record's rows: a pair's is the unit's; the second stream of the same pairs keeps what it puts by 128 rows further down, which no pair has then.
+      float* const rows = a.acc + static_cast<size_t>(max(s.block, 0)) * kPrefixTcPairs * a.d8;
+      float* const put = rows + static_cast<size_t>(w * kRows + r) * a.d8 + h * kCols;
+      const int put_cols = a.d8 - h * kCols;
+      float top = -INFINITY, sum = 0.f, put_top = -INFINITY;
+      for (int i = 0; i < count; ++i) {
+        const int live = steps.live(w, i);
+        ok = MbarWaitWarp(sfull + 8 * w, (steps_done + i) & 1, lane, abort_word) && ok;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        if ((live & 15) != 0 && (split || w == 0)) {
+        if ((live & 15) != 0 && (!steps.pair_tiles || w == 0)) {
           // Values behind the end in the last 16 that are multiplied: 0 times whatever the page holds there must stay 0.
-          const int it = items + ValueItem(split, n, t), sl = it % kSlots;
+          const int it = items + 2 * i + 1, sl = it % kSlots;
           ok = MbarWaitWarp(full + 8 * sl, (it / kSlots) & 1, lane, abort_word) && ok;
-          const int dead = 16 - (live & 15);
-          for (int i = r; i < dead * kChunks; i += kRows) {
-            const int c = i / dead, row = live + i % dead;
+          const int dead = 16 - (live & 15), first = steps.first(w) + live;
+          for (int k = h * kRows + r; k < dead * kChunks; k += 2 * kRows) {
+            const int c = k / dead, row = first + k % dead;
             Store32(ring + sl * kPart + (c >> 3) * kAtom + row * 128 + ((c & 7) << 4), make_uint4(0u, 0u, 0u, 0u));
           }
           FenceAsync();
         }
         if (live_warp) {
-          uint32_t x[kKeys];
+          // All but the last 32 scores are read twice: kept between their maximum and their weights they would cost more registers than sixteen warps have.
+          auto scores = [&](int c, float* x) {
+            TcLd32(sa + 32 * c, reinterpret_cast<uint32_t*>(x));
+            asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+            const int n = live - (h * chunks + c) * 32;
+            if (n < 32) {
 #pragma unroll
-          for (int c = 0; c < kKeys; c += 32) TcLd32(sa + c, x + c);
-          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-          if (live < kKeys) {
+              for (int e = 0; e < 32; ++e)
+                if (e >= n) x[e] = -INFINITY;
+            }
+          };
+          float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, x[32];
+#pragma unroll 1
+          for (int c = 0; c < chunks; ++c) {
+            scores(c, x);
 #pragma unroll
-            for (int e = 0; e < kKeys; ++e)
-              if (e >= live) x[e] = 0xff800000u;
+            for (int e = 0; e < 32; e += 2) t4[(e >> 1) & 3] = Max3(t4[(e >> 1) & 3], x[e], x[e + 1]);
           }
-          float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float step_top = Max3(Max3(t4[0], t4[1], t4[2]), t4[3], -INFINITY) * scale_log2;
+          const bool flush = PLO && i > 0 && i % kChain == 0;
+          const bool raise = EitherWarp(meet, step_top > top + kLazy || (top == -INFINITY && step_top > -INFINITY));
+          if (flush) {  // the product before these scores is done: O has every step before this one in it
+            const float keep = put_top == -INFINITY ? 0.f : Exp2(put_top - top);
+#pragma unroll 1
+            for (int c = 0; c < kCols; c += 16) {
+              float o[16];
+              TcLd16(oh + c, reinterpret_cast<uint32_t*>(o));
+              asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
-          for (int e = 0; e < kKeys; ++e) t4[e & 3] = fmaxf(t4[e & 3], __uint_as_float(x[e]));
-          const float tile_top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * scale_log2;
-          if (__any_sync(0xffffffffu, tile_top > top + kLazy || (top == -INFINITY && tile_top > -INFINITY))) {
-            const float next = fmaxf(top, tile_top), keep = top == -INFINITY ? 0.f : Exp2(top - next);
-            if (j > 0) {  // O has every tile before this one in it: their products were ahead of these scores
+              for (int e = 0; e < 16; e += 8) {
+                if (!mine || c + e >= put_cols) continue;
+                if (i > kChain) {
 #pragma unroll
-              for (int c = 0; c < ATOMS * 64; c += 32) {
-                uint32_t o[32];
-                TcLd32(oa + w * 128 + c, o);
+                  for (int k = 0; k < 8; ++k) o[e + k] = fmaf(put[c + e + k], keep, o[e + k]);
+                }
+                StoreSector(put + c + e, o + e);
+              }
+            }
+            put_top = top;
+          }
+          if (raise) {
+            // One maximum for both halves of the scores.
+            if (h == 0) s_top[w][r] = step_top;
+            WarpsSync(meet);
+            if (h == 1) s_top[w][r] = step_top = fmaxf(step_top, s_top[w][r]);
+            WarpsSync(meet);
+            if (h == 0) step_top = s_top[w][r];
+            const float next = fmaxf(top, step_top), keep = top == -INFINITY ? 0.f : Exp2(top - next);
+            if (i > 0 && !flush) {
+#pragma unroll 1
+              for (int c = 0; c < kCols; c += 16) {
+                uint32_t o[16];
+                TcLd16(oh + c, o);
                 asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                TcSt32(oa + w * 128 + c, o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                TcSt16(oh + c, o);
               }
             }
             sum *= keep;
             top = next;
           }
           const float ref = top == -INFINITY ? 0.f : top;
-          float s4[4] = {};
+          const uint64_t scale2 = Both(scale_log2, scale_log2), ref2 = Both(-ref, -ref);
+          uint64_t s2[2] = {0ull, 0ull};
+#pragma unroll 1
+          for (int c = chunks - 1; c >= 0; --c) {  // a chunk's weights take its place: 16 columns, and 16 of what they lose as bf16
+            if (c + 1 < chunks) scores(c, x);
+            uint32_t hi[16], lo[PLO ? 16 : 1];
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {  // 64 keys: 32 columns of weights, and 32 of what they lose as bf16
-            uint32_t hi[32], lo[PLO ? 32 : 1];
-#pragma unroll
-            for (int e = 0; e < 64; e += 2) {
-              const float p0 = Exp2(fmaf(__uint_as_float(x[64 * half + e]), scale_log2, -ref)), p1 = Exp2(fmaf(__uint_as_float(x[64 * half + e + 1]), scale_log2, -ref));
-              s4[e & 2] += p0;
-              s4[(e & 2) + 1] += p1;
+            for (int e = 0; e < 32; e += 2) {
+              float p0, p1;
+              Apart(Fma2(Both(x[e], x[e + 1]), scale2, ref2), p0, p1);
+              p0 = Exp2(p0);
+              p1 = Exp2(p1);
+              s2[(e >> 1) & 1] = Add2(s2[(e >> 1) & 1], Both(p0, p1));
               hi[e / 2] = Pack(p0, p1);
               if constexpr (PLO) lo[e / 2] = Pack(p0 - Low(hi[e / 2]), p1 - High(hi[e / 2]));
             }
-            TcSt32(sa + 32 * half, hi);
-            if constexpr (PLO) TcSt32(sa + 64 + 32 * half, lo);
+            TcSt16(sa + 32 * c, hi);
+            if constexpr (PLO) TcSt16(sa + 32 * c + 16, lo);
           }
-          sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+          float s0, s1;
+          Apart(Add2(s2[0], s2[1]), s0, s1);
+          sum += s0 + s1;
           asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
         }
         asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -348,56 +467,74 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = MbarWaitWarp(odone + 8 * w, segments & 1, lane, abort_word) && ok;
         ++segments;
       }
+      asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+      SoftmaxWarpsSync();  // every product is done: the queries' place is free
+      // A pair's threads tell each other their sums, and what was put by counts now.
+      float4* const told = reinterpret_cast<float4*>(smem);  // [stream][half][row]
+      const float kept = PLO && count > kChain && put_top != -INFINITY ? Exp2(put_top - top) : 0.f;
+      told[(w * 2 + h) * kRows + r] = make_float4(top, sum, kept, 0.f);
+      SoftmaxWarpsSync();
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-      const size_t rec = static_cast<size_t>(max(s.block, 0)) * kPrefixTcPairs + (pair_tiles ? w * kRows : 0) + r;
-      const bool mine = s.block >= 0 && (pair_tiles ? w * kRows : 0) + r < s.pairs;
-      float* out = a.acc + rec * a.d8;
-      if (!split) {
-        if (mine && (pair_tiles || w == 0)) *reinterpret_cast<float2*>(a.heads + 2 * rec) = make_float2(RecordMax(top * kLn2, sum), sum);
-        if (live_warp && (pair_tiles || w == 0)) {
+      float2* const head = reinterpret_cast<float2*>(a.heads) + static_cast<size_t>(max(s.block, 0)) * kPrefixTcPairs + own_pair;
+      float* const out = rows + static_cast<size_t>(own_pair) * a.d8;
+      if (steps.pair_tiles) {
+        const float all = sum + told[(w * 2 + (h ^ 1)) * kRows + r].y;
+        if (mine && h == 0) *head = make_float2(RecordMax(top * kLn2, all), all);
+        if (live_warp) {
 #pragma unroll
-          for (int c = 0; c < ATOMS * 64; c += 32) {
-            float o[32];
-            TcLd32(oa + w * 128 + c, reinterpret_cast<uint32_t*>(o));
+          for (int c = 0; c < kCols; c += 16) {
+            float o[16];
+            TcLd16(oh + c, reinterpret_cast<uint32_t*>(o));
             asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              if (mine && c + e < a.d8) StoreSector(out + c + e, o + e);
+            for (int e = 0; e < 16; e += 8) {
+              if (!mine || c + e >= put_cols) continue;
+              if (PLO && count > kChain) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) o[e + k] = fmaf(put[c + e + k], kept, o[e + k]);
+              }
+              StoreSector(put + c + e, o + e);
+            }
           }
         }
       } else {
-        // Both streams have these pairs: each takes half of the channels of both.  They meet where a second tile of queries would lie.
-        float2* both = reinterpret_cast<float2*>(smem + Layout::kQTile);
-        if (sum != sum) top = sum;  // no score was a number: the record is not one either
-        both[w * kRows + r] = make_float2(top, sum);
-        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-        SoftmaxWarpsSync();
-        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        const float2 other = both[(w ^ 1) * kRows + r];
-        const float ref = fmaxf(top, other.x);
-        const float f_mine = top == -INFINITY ? 0.f : Exp2(top - ref), f_other = other.x == -INFINITY ? 0.f : Exp2(other.x - ref);
-        const float f0 = w == 0 ? f_mine : f_other, f1 = w == 0 ? f_other : f_mine;
-        const float all = sum * f_mine + other.y * f_other;
-        if (mine && w == 0) *reinterpret_cast<float2*>(a.heads + 2 * rec) = make_float2(RecordMax(ref * kLn2, all), all);
+        // Both streams have these pairs: each of the four threads of a pair takes a quarter of the channels of both.
+        float4 h0 = told[r], h1 = told[2 * kRows + r];
+        h0.y += told[kRows + r].y;
+        h1.y += told[3 * kRows + r].y;
+        if (h0.y != h0.y) h0.x = h0.y;  // no score was a number: the record is not one either
+        if (h1.y != h1.y) h1.x = h1.y;
+        const float ref = fmaxf(h0.x, h1.x), f0 = h0.x == -INFINITY ? 0.f : Exp2(h0.x - ref), f1 = h1.x == -INFINITY ? 0.f : Exp2(h1.x - ref);
+        const float all = h0.y * f0 + h1.y * f1;
+        if (mine && w == 0 && h == 0) *head = make_float2(RecordMax(ref * kLn2, all), all);
         if (live_warp) {
-#pragma unroll
-          for (int c = 0; c < ATOMS * 32; c += 32) {
-            const int col = w * ATOMS * 32 + c;
-            float o[32], o1[32];
-            TcLd32(oa + col, reinterpret_cast<uint32_t*>(o));
-            TcLd32(oa + 128 + col, reinterpret_cast<uint32_t*>(o1));
+          const int first = (w * 2 + h) * (kCols / 2);
+#pragma unroll 1
+          for (int c = first; c < first + kCols / 2; c += 16) {
+            float o[16], o1[16];
+            TcLd16(oa + c, reinterpret_cast<uint32_t*>(o));
+            TcLd16(oa + 128 + c, reinterpret_cast<uint32_t*>(o1));
             asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = o[e] * f0 + o1[e] * f1;
+            for (int e = 0; e < 16; e += 8) {
+              if (!mine || c + e >= a.d8) continue;
 #pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              if (mine && col + e < a.d8) StoreSector(out + col + e, o + e);
+              for (int k = 0; k < 8; ++k) {
+                if constexpr (PLO) {
+                  if (steps.count(0) > kChain) o[e + k] = fmaf(out[c + e + k], h0.z, o[e + k]);
+                  if (steps.count(1) > kChain) o1[e + k] = fmaf(out[static_cast<size_t>(kRows) * a.d8 + c + e + k], h1.z, o1[e + k]);
+                }
+                o[e + k] = (f0 == 0.f ? 0.f : o[e + k] * f0) + (f1 == 0.f ? 0.f : o1[e + k] * f1);  // a stream without steps has no outputs
+              }
+              StoreSector(out + c + e, o + e);
+            }
           }
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-      SoftmaxWarpsSync();  // accumulators and queries of this segment are read: the next one's may come
-      items += 2 * n;
+      SoftmaxWarpsSync();  // accumulators and what was told in the queries' place are read: the next segment's may come
+      items += 2 * steps.n;
+      steps_done += count;
     }
   }
   if (!ok) atomicExch(&g_prefix_status, 1);
