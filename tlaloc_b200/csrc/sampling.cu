@@ -4,15 +4,27 @@
 //   w_i = exp((x_i - max x) / T);  kept: rank_i < k,  mass of the better ranked < p * mass of the k,  w_i >= min_p
 //   token = first i whose running sum of kept w, in index order, exceeds u * their whole sum
 //
-// Ranks go by value, equal values by index.  So what is kept is all values above some value and, of those equal to it, the ones up to some index.
-// Weights and sums are f64: a row has as many borders between tokens as it has tokens, and a draw that sums 10^5 weights in f32 lands on the wrong side of one in
-// about one row of a hundred.
+// Ranks go by value, equal values by index.  So what is kept is all values above some edge and, of those equal to it, the ones up to some index; the edges of top-k and
+// top-p are found without sorting the row.  Weights and sums are f64: a row has as many borders between tokens as it has tokens, and a draw that sums 10^5 weights in f32
+// lands on the wrong side of one in about one row of a hundred.
+//
+// A cluster of CTAs shares a row; each reads its part once and keeps it in shared memory where it fits.  Passes over the part:
+//   1  the largest value
+//   2  (with top-k or top-p) how many values, and roughly which mass, lie in each of 1024 bins of (max - x) / T, and the exact mass of all
+//   3  per edge: the exact count and mass above the bin that it lies in; the bin's values go to one CTA, which ranks them and finds the edge.  The rough masses of
+//      pass 2 only say where to look: the exact ones decide, and move on to a neighbouring bin if they must.  A bin with more values than a CTA holds is halved by
+//      value, over and over (equal logits by the thousand)
+//   4  the mass that is kept, by warp, and then the draw, in the one warp whose stretch it falls into
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "common.cuh"
 
 namespace tlaloc_b200 {
 namespace {
+
+namespace cg = cooperative_groups;
 
 struct SampleArgs {
   const void* logits;
@@ -25,10 +37,14 @@ struct SampleArgs {
   float temperature_all, top_p_all, min_p_all;
   int top_k_all;
   int* out;
-  int n;
+  int n, per;  // values of a row, and of a CTA's part
+  int on_chip;
 };
 
-constexpr int kSampleThreads = 1024, kSampleWarps = kSampleThreads / 32;
+constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
+constexpr int kBins = 1024, kMaxRanks = 8;
+constexpr float kBinsPerOctave = 16.f;  // of w: the last bin begins 64 octaves below the largest
+constexpr int kRanked = 512;            // values of a bin that one CTA ranks
 
 // Values in an order of unsigned numbers: -0 as 0, NaN as -infinity (never drawn).
 __device__ __forceinline__ uint32_t KeyOf(float x)
@@ -39,191 +55,554 @@ __device__ __forceinline__ uint32_t KeyOf(float x)
 }
 __device__ __forceinline__ float ValueOf(uint32_t key) { return __uint_as_float(key ^ ((key >> 31) != 0u ? 0x80000000u : 0xffffffffu)); }
 
-template <typename T>
-__device__ __forceinline__ T BlockSumAll(T v, T* red)
+// exp(d) for d <= 0 by a table of 2^(j / 256) and a polynomial of degree 4 in what is left, |r| <= ln 2 / 512 (Tang, "Table-driven implementation of the exponential function",
+// 1989): the first term left out is r^5 / 120 = 4e-17 of the result.  Nine f64 operations instead of the library's twenty; below 2^-1000 the result is 0.
+constexpr int kExpTable = 256;
+__device__ __forceinline__ double TableExp2(double t, const double* table)  // 2^t, t <= 0
 {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  T r = 0;
-  for (int w = 0; w < kSampleWarps; ++w) r += red[w];
-  return r;
+  if (t < -1000.0) return 0.0;
+  constexpr double kRound = 6755399441055744.0 / kExpTable;  // 1.5 * 2^52 / 256: its last place is 1 / 256
+  const double shifted = t + kRound;
+  const int k = __double2loint(shifted);  // t * 256 rounded, in the low word
+  const double r = (t - (shifted - kRound)) * 0.69314718055994530942;
+  const double p = fma(fma(fma(fma(r, 1.0 / 24, 1.0 / 6), r, 0.5), r, 1.0), r, 1.0);
+  const double scaled = table[k & (kExpTable - 1)] * p;
+  return __hiloint2double(__double2hiint(scaled) + ((k >> 8) << 20), __double2loint(scaled));
 }
 
 template <typename XT>
 __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_constant__ SampleArgs a)
 {
+  extern __shared__ __align__(16) unsigned char part_raw[];  // this CTA's part of the row, where it fits
+  __shared__ double table[kExpTable];
+  __shared__ double red[kSampleWarps], told_mass[kMaxRanks], warp_mass[kSampleWarps];
+  __shared__ int ired[kSampleWarps], told_count[kMaxRanks];
+  __shared__ uint32_t kred[kSampleWarps], told_key[kMaxRanks];
+  __shared__ int bin_count[kBins];
+  __shared__ float bin_mass[kBins];
+  __shared__ uint32_t cand_key[kRanked];
+  __shared__ int cand_index[kRanked];
+  __shared__ int cand_n;
+  __shared__ struct {
+    uint32_t key;
+    int index;
+  } edge_s;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank()), ranks = static_cast<int>(cluster.num_blocks());
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x;
+  if (ranks > 1) cluster.barrier_arrive();  // waited for ahead of the first write into another rank's memory
+  for (int i = tid; i < kExpTable; i += kSampleThreads) table[i] = exp2(static_cast<double>(i) / kExpTable);
   GridDependencySync();
-  __shared__ double red[kSampleWarps];
-  __shared__ int ired[kSampleWarps];
-  __shared__ uint32_t kred[kSampleWarps];
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n;
-  const XT* x = static_cast<const XT*>(a.logits) + row * a.ld;
+  const int lo = min(rank * a.per, a.n), n = min(lo + a.per, a.n) - lo;  // this CTA's part: [lo, lo + n)
+  const XT* x = static_cast<const XT*>(a.logits) + row * a.ld + lo;
   const float temperature = a.temperature != nullptr ? __ldg(a.temperature + row) : a.temperature_all;
   const int top_k = a.top_k != nullptr ? __ldg(a.top_k + row) : a.top_k_all;
   const float top_p = a.top_p != nullptr ? __ldg(a.top_p + row) : a.top_p_all;
   const float min_p = a.min_p != nullptr ? __ldg(a.min_p + row) : a.min_p_all;
-  const int per = (n + kSampleWarps - 1) / kSampleWarps;  // a warp's stretch of the row
-  const int lo = min(warp * per, n), hi = min(lo + per, n);
+  const float u = __ldg(a.uniforms + row);
 
-  // The largest value, and the first place of it.
+  // Sums over the block, and over the cluster in rank order: the same for every thread.
+  auto block_sum = [&](auto v, auto* buffer) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if (lane == 0) buffer[warp] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < kSampleWarps; ++w) v += buffer[w];
+    return v;
+  };
+  auto cluster_sum = [&](auto v, auto* buffer, auto* told) {
+    v = block_sum(v, buffer);
+    if (ranks == 1) return v;
+    if (tid < ranks) *cluster.map_shared_rank(told + rank, tid) = v;
+    cluster.sync();
+    v = 0;
+    for (int q = 0; q < ranks; ++q) v += told[q];
+    cluster.sync();  // read by all: the next one may be told
+    return v;
+  };
+
+  // 1: the largest value, and the part into shared memory.
+  XT* const part = reinterpret_cast<XT*>(part_raw);
   uint32_t best = 0;
-  for (int i = lo + lane; i < hi; i += 32) best = max(best, KeyOf(ToF32(x[i])));
+  {
+    constexpr int kPer = 16 / static_cast<int>(sizeof(XT));
+    const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    const int words = vec ? n / kPer : 0;
+    constexpr int kAhead = 4;
+    for (int i0 = tid; i0 < words; i0 += kSampleThreads * kAhead) {
+      uint4 raw[kAhead];
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e)
+        if (i0 + e * kSampleThreads < words) raw[e] = __ldcg(reinterpret_cast<const uint4*>(x) + i0 + e * kSampleThreads);
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        if (i0 + e * kSampleThreads >= words) continue;
+        if (a.on_chip) reinterpret_cast<uint4*>(part)[i0 + e * kSampleThreads] = raw[e];
+        const XT* v = reinterpret_cast<const XT*>(&raw[e]);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) best = max(best, KeyOf(ToF32(v[k])));
+      }
+    }
+    for (int i = words * kPer + tid; i < n; i += kSampleThreads) {
+      const XT v = x[i];
+      if (a.on_chip) part[i] = v;
+      best = max(best, KeyOf(ToF32(v)));
+    }
+  }
+  const XT* const v = a.on_chip ? part : x;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
   if (lane == 0) kred[warp] = best;
-  __syncthreads();
+  __syncthreads();  // the part is there, too
   for (int w = 0; w < kSampleWarps; ++w) best = max(best, kred[w]);
+  if (ranks > 1) {
+    cluster.barrier_wait();
+    if (tid < ranks) *cluster.map_shared_rank(told_key + rank, tid) = best;
+    cluster.sync();
+    for (int q = 0; q < ranks; ++q) best = max(best, told_key[q]);
+  }
   const float top = ValueOf(best);
+  const int chunk = ((n + kSampleWarps - 1) / kSampleWarps + 31) / 32 * 32;  // a warp's stretch of the part
+  const int w_lo = min(warp * chunk, n), w_hi = min(w_lo + chunk, n);
+
   if (!(temperature > 0.f) || top == -INFINITY) {  // greedy, or nothing to draw: the first of the largest, index 0 of a row without one
     int at = 0x7fffffff;
-    for (int i = lo + lane; i < hi; i += 32)
-      if (KeyOf(ToF32(x[i])) == best) at = min(at, i);
+    for (int i = tid; i < n; i += kSampleThreads)
+      if (KeyOf(ToF32(v[i])) == best) at = min(at, lo + i);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
     if (lane == 0) ired[warp] = at;
     __syncthreads();
     for (int w = 0; w < kSampleWarps; ++w) at = min(at, ired[w]);
-    if (tid == 0) a.out[row] = top == -INFINITY ? 0 : at;
+    if (ranks > 1) {
+      if (tid == 0) *cluster.map_shared_rank(told_count + rank, 0) = at;
+      cluster.sync();
+      if (rank == 0)
+        for (int q = 0; q < ranks; ++q) at = min(at, told_count[q]);
+    }
+    if (rank == 0 && tid == 0) a.out[row] = top == -INFINITY ? 0 : at;
     return;
   }
-  const double inv = 1.0 / static_cast<double>(temperature), dtop = static_cast<double>(top);
-  auto weight = [&](uint32_t key) -> double {
-    const float v = ValueOf(key);
-    if (v == top) return 1.0;
-    if (v == -INFINITY || top == INFINITY) return 0.0;
-    return exp((static_cast<double>(v) - dtop) * inv);
+
+  const double scale = 1.4426950408889634074 / static_cast<double>(temperature), dtop = static_cast<double>(top);
+  auto weight = [&](float f) -> double {
+    if (f == top) return 1.0;
+    if (!(f > -INFINITY) || top == INFINITY) return 0.0;
+    return TableExp2((static_cast<double>(f) - dtop) * scale, table);
   };
-  auto count_from = [&](uint32_t key) {  // how many are as large as `key` or larger
-    int c = 0;
-    for (int i = lo + lane; i < hi; i += 32) c += KeyOf(ToF32(x[i])) >= key ? 1 : 0;
-    return BlockSumAll(c, ired);
+  // The bin of a value: a function that does not rise with it, however it is rounded.
+  const float fscale = fminf(static_cast<float>(scale) * kBinsPerOctave, 3.0e38f);
+  auto bin_of = [&](float f) -> int {
+    if (f == top) return 0;
+    if (!(f > -INFINITY) || top == INFINITY) return kBins - 1;
+    return static_cast<int>(fminf((top - f) * fscale, static_cast<float>(kBins - 1)));
   };
-  auto mass_from = [&](uint32_t key) {  // and their mass
-    double m = 0.0;
-    for (int i = lo + lane; i < hi; i += 32) {
-      const uint32_t k = KeyOf(ToF32(x[i]));
-      if (k >= key) m += weight(k);
+
+  // Kept: keys above edge_key, and of those equal to it the ones up to edge_index.
+  uint32_t edge_key = 0;
+  int edge_index = a.n;
+  const bool by_k = top_k > 0 && top_k < a.n, by_p = top_p < 1.f;
+  if (by_k || by_p) {
+    // 2: the bins, and the mass of all.
+    for (int i = tid; i < kBins; i += kSampleThreads) {
+      bin_count[i] = 0;
+      bin_mass[i] = 0.f;
     }
-    return BlockSumAll(m, red);
-  };
-  // Kept: keys above `edge`, and the first `quota` of those equal to it.
-  uint32_t edge = 0;
-  int quota = n;
-  double mass = 0.0;
-  const bool by_k = top_k > 0 && top_k < n, by_p = top_p < 1.f;
-  if (by_k) {  // the largest key that k are as large as
-    uint32_t a0 = 0, a1 = best;
-    while (a0 < a1) {
-      const uint32_t mid = a0 + (a1 - a0 + 1) / 2;
-      if (count_from(mid) >= top_k) a0 = mid;
-      else a1 = mid - 1;
-    }
-    edge = a0;
-    quota = top_k - (edge == best ? 0 : count_from(edge + 1));
-  }
-  if (by_p) {
-    mass = by_k ? (edge == best ? 0.0 : mass_from(edge + 1)) + quota * weight(edge) : mass_from(0);
-    const double share = fmax(static_cast<double>(top_p), 0.0) * mass;
-    // The smallest key whose betters hold less than the share; the best one always does.
-    uint32_t a0 = edge, a1 = best;
-    while (a0 < a1) {
-      const uint32_t mid = a0 + (a1 - a0) / 2;
-      if (mass_from(mid + 1) < share) a1 = mid;
-      else a0 = mid + 1;
-    }
-    const double above = a0 == best ? 0.0 : mass_from(a0 + 1), w = weight(a0);
-    if (a0 != edge) quota = n;
-    // The j-th of the equal ones stays while above + j w < share.
-    if (w > 0.0) {
-      double most = ceil((share - above) / w);
-      if (most > 1.0 && above + (most - 1.0) * w >= share) most -= 1.0;
-      if (above + most * w < share) most += 1.0;
-      quota = static_cast<int>(fmin(static_cast<double>(quota), fmax(most, 1.0)));
-    }
-    edge = a0;
-  }
-  // Up to which place the equal ones stay.
-  int equal = 0;
-  for (int i = lo + lane; i < hi; i += 32) equal += KeyOf(ToF32(x[i])) == edge ? 1 : 0;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) equal += __shfl_xor_sync(0xffffffffu, equal, o);
-  __syncthreads();
-  if (lane == 0) ired[warp] = equal;
-  __syncthreads();
-  int before = 0;
-  for (int w = 0; w < warp; ++w) before += ired[w];
-  const double least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
-  // A warp walks its stretch in order, 32 at a time; what(i, w) gets every kept place of a lane and its weight (0 for the others).
-  auto walk = [&](auto&& what) {
-    int seen = before;
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-      const int i = i0 + lane;
-      const uint32_t key = i < hi ? KeyOf(ToF32(x[i])) : 0u;
-      const unsigned ties = __ballot_sync(0xffffffffu, i < hi && key == edge);
-      const bool in = i < hi && (key > edge || (key == edge && seen + __popc(ties & ((1u << lane) - 1u)) < quota));
-      seen += __popc(ties);
-      double w = 0.0;
-      if (in) {
-        w = weight(key);
-        if (w < least) w = 0.0;
+    __syncthreads();
+    double all = 0.0;
+    for (int i = tid; i < n; i += kSampleThreads) {
+      const float f = ToF32(v[i]);
+      const int b = bin_of(f);
+      atomicAdd(&bin_count[b], 1);
+      if (by_p) {
+        const double w = weight(f);
+        all += w;
+        atomicAdd(&bin_mass[b], static_cast<float>(w));
       }
-      if (what(i, w)) return;
     }
+    if (by_p) all = cluster_sum(all, red, told_mass);
+    else __syncthreads();
+    if (ranks > 1) {  // the row's bins: every rank adds up an equal share of them over all ranks and tells everyone
+      cluster.sync();
+      const int share = kBins / ranks, b = rank * share + tid;
+      int c = 0;
+      float m = 0.f;
+      if (tid < share) {
+        for (int q = 0; q < ranks; ++q) {
+          c += *cluster.map_shared_rank(bin_count + b, q);
+          m += *cluster.map_shared_rank(bin_mass + b, q);
+        }
+      }
+      cluster.sync();
+      if (tid < share) {
+        for (int q = 0; q < ranks; ++q) {
+          *cluster.map_shared_rank(bin_count + b, q) = c;
+          *cluster.map_shared_rank(bin_mass + b, q) = m;
+        }
+      }
+      cluster.sync();
+    }
+    // The first bin at whose end `enough(count, mass)` holds; the last one if it never does.
+    auto find_bin = [&](auto&& enough) {
+      __shared__ int found_s;
+      __shared__ int cs[kSampleWarps];
+      __shared__ float ms[kSampleWarps];
+      constexpr int kEach = kBins / kSampleThreads;
+      int c[kEach];
+      float m[kEach];
+      int ct = 0;
+      float mt = 0.f;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        ct += bin_count[tid * kEach + e];
+        mt += bin_mass[tid * kEach + e];
+        c[e] = ct;
+        m[e] = mt;
+      }
+      int cu = ct;
+      float mu = mt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int cc = __shfl_up_sync(0xffffffffu, cu, o);
+        const float mm = __shfl_up_sync(0xffffffffu, mu, o);
+        if (lane >= o) {
+          cu += cc;
+          mu += mm;
+        }
+      }
+      __syncthreads();
+      if (tid == 0) found_s = kBins - 1;
+      if (lane == 31) {
+        cs[warp] = cu;
+        ms[warp] = mu;
+      }
+      __syncthreads();
+      int cb = cu - ct;
+      float mb = mu - mt;
+      for (int w = 0; w < warp; ++w) {
+        cb += cs[w];
+        mb += ms[w];
+      }
+#pragma unroll
+      for (int e = kEach - 1; e >= 0; --e)
+        if (enough(cb + c[e], mb + m[e])) atomicMin(&found_s, tid * kEach + e);
+      __syncthreads();
+      const int b = found_s;
+      __syncthreads();
+      return b;
+    };
+
+    // 3: the edge in or next to bin `b`.  Counting: the value of rank `want_count`.  Otherwise: the last value whose betters hold less than `want_mass`, none beyond
+    // (limit_key, limit_index).  kept_mass, if given: the exact mass of what is kept.
+    auto find_edge = [&](int b, bool counting, int want_count, double want_mass, uint32_t limit_key, int limit_index, double* kept_mass) {
+      int moved = 0;  // which way: never back, whatever sums of the same values in two groupings say
+      for (;;) {
+        // Exactly what lies above the bin, and in it.
+        int above_n = 0, in_n = 0;
+        double above = 0.0, in = 0.0;
+        for (int i = tid; i < n; i += kSampleThreads) {
+          const float f = ToF32(v[i]);
+          const int at = bin_of(f);
+          if (at > b) continue;
+          const uint32_t key = KeyOf(f);
+          if (key < limit_key || (key == limit_key && lo + i > limit_index)) continue;
+          const double w = weight(f);
+          if (at < b) {
+            ++above_n;
+            above += w;
+          } else {
+            ++in_n;
+            in += w;
+          }
+        }
+        above_n = cluster_sum(above_n, ired, told_count);
+        in_n = cluster_sum(in_n, ired, told_count);
+        above = cluster_sum(above, red, told_mass);
+        in = cluster_sum(in, red, told_mass);
+        if (!counting && above_n > 0 && above >= want_mass) {  // roundings of the rough masses: the edge lies higher
+          if (moved <= 0) {
+            moved = -1;
+            --b;
+            continue;
+          }
+          want_mass = above * (1.0 + 1e-15);
+        }
+        if (!counting && above + in < want_mass && moved >= 0 && b + 1 < kBins) {
+          moved = 1;
+          ++b;
+          continue;
+        }
+        if (in_n == 0) return;  // all of them stay
+        // The bin's values between these keys, while they are too many for one CTA: halved by value.
+        uint32_t k_lo = 0, k_hi = 0xffffffffu;
+        while (in_n > kRanked && k_lo < k_hi) {
+          const uint32_t mid = k_lo + (k_hi - k_lo) / 2;  // the upper half: keys above it
+          int up_n = 0;
+          double up = 0.0;
+          for (int i = tid; i < n; i += kSampleThreads) {
+            const float f = ToF32(v[i]);
+            const uint32_t key = KeyOf(f);
+            if (key <= mid || key > k_hi || bin_of(f) != b || key < limit_key || (key == limit_key && lo + i > limit_index)) continue;
+            ++up_n;
+            up += weight(f);
+          }
+          up_n = cluster_sum(up_n, ired, told_count);
+          up = cluster_sum(up, red, told_mass);
+          // Neither half is taken empty.
+          const bool higher = up_n > 0 && (up_n == in_n || (counting ? above_n + up_n >= want_count : above + up >= want_mass));
+          if (higher) {
+            k_lo = mid + 1;
+            in_n = up_n;
+          } else {
+            k_hi = mid;
+            in_n -= up_n;
+            above_n += up_n;
+            above += up;
+          }
+        }
+        if (in_n > kRanked) {  // that many equal values: the edge is one of them, by how many there is room for
+          const uint32_t key = k_lo;
+          const double w = weight(ValueOf(key));
+          int quota = in_n;
+          if (counting) {
+            quota = want_count - above_n;
+          } else if (w > 0.0) {  // the j-th stays while above + j w < want
+            double most = ceil((want_mass - above) / w);
+            if (most > 1.0 && above + (most - 1.0) * w >= want_mass) most -= 1.0;
+            if (above + most * w < want_mass) most += 1.0;
+            quota = static_cast<int>(fmin(static_cast<double>(in_n), fmax(most, 1.0)));
+          }
+          // The index of the quota-th of them: equal ones of the ranks before, of the warps before, then by 32.
+          int equal = 0;
+          for (int i = w_lo + lane; i < w_hi; i += 32) equal += KeyOf(ToF32(v[i])) == key ? 1 : 0;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) equal += __shfl_xor_sync(0xffffffffu, equal, o);
+          __syncthreads();
+          if (lane == 0) ired[warp] = equal;
+          __syncthreads();
+          int before = 0, mine = 0;
+          for (int w2 = 0; w2 < kSampleWarps; ++w2) {
+            if (w2 < warp) before += ired[w2];
+            mine += ired[w2];
+          }
+          if (ranks > 1) {
+            if (tid < ranks) *cluster.map_shared_rank(told_count + rank, tid) = mine;
+            cluster.sync();
+            for (int q = 0; q < rank; ++q) before += told_count[q];
+          }
+          if (before < quota && before + equal >= quota) {
+            int seen = before;
+            for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
+              const bool is = i0 + lane < w_hi && KeyOf(ToF32(v[i0 + lane])) == key;
+              const unsigned ties = __ballot_sync(0xffffffffu, is);
+              if (is && seen + __popc(ties & ((1u << lane) - 1u)) + 1 == quota) {
+                for (int q = 0; q < ranks; ++q) cluster.map_shared_rank(&edge_s, q)->index = lo + i0 + lane;
+              }
+              seen += __popc(ties);
+            }
+          }
+          cluster.sync();
+          edge_key = key;
+          edge_index = edge_s.index;
+          if (kept_mass != nullptr) *kept_mass = above + quota * w;
+          cluster.sync();
+          return;
+        }
+        // The values of the bin (or of what is left of it) in rank 0, in any order.
+        if (tid == 0) cand_n = 0;
+        cluster.sync();
+        int* const count0 = cluster.map_shared_rank(&cand_n, 0);
+        uint32_t* const key0 = cluster.map_shared_rank(cand_key, 0);
+        int* const index0 = cluster.map_shared_rank(cand_index, 0);
+        for (int i = tid; i < n; i += kSampleThreads) {
+          const float f = ToF32(v[i]);
+          const uint32_t key = KeyOf(f);
+          if (bin_of(f) != b || key < k_lo || key > k_hi || key < limit_key || (key == limit_key && lo + i > limit_index)) continue;
+          const int at = atomicAdd(count0, 1);
+          key0[at] = key;
+          index0[at] = lo + i;
+        }
+        cluster.sync();
+        if (rank == 0) {
+          // Each value's betters among them, their number and mass: the edge is the one whose betters leave room and which itself takes the last of it.
+          const int m = cand_n;
+          for (int i = tid; i < m; i += kSampleThreads) {
+            const uint32_t key = cand_key[i];
+            const int index = cand_index[i];
+            int better = 0;
+            for (int j = 0; j < m; ++j) better += cand_key[j] > key || (cand_key[j] == key && cand_index[j] < index) ? 1 : 0;
+            // by rank, into the bins' place: they are no longer needed by this CTA once the edge is known
+            if (counting ? above_n + better + 1 == want_count : false) {
+              edge_s.key = key;
+              edge_s.index = index;
+            }
+            if (!counting) reinterpret_cast<int*>(bin_mass)[better] = i;
+          }
+          __syncthreads();
+          if (!counting && warp == 0) {  // running sums by rank, 32 at a time
+            double run = above;
+            int last = 0;
+            bool over = false;
+            for (int j0 = 0; j0 < m && !over; j0 += 32) {
+              const int at = j0 + lane < m ? reinterpret_cast<int*>(bin_mass)[j0 + lane] : 0;
+              const double w = j0 + lane < m ? weight(ValueOf(cand_key[at])) : 0.0;
+              double up = w;
+#pragma unroll
+              for (int o = 1; o < 32; o <<= 1) {
+                const double t = __shfl_up_sync(0xffffffffu, up, o);
+                if (lane >= o) up += t;
+              }
+              double in_front = __shfl_up_sync(0xffffffffu, up, 1);
+              if (lane == 0) in_front = 0.0;
+              const bool stays = j0 + lane < m && (run + in_front < want_mass || (above_n == 0 && j0 + lane == 0));
+              const unsigned stay = __ballot_sync(0xffffffffu, stays);
+              if (stay != 0u) last = j0 + 31 - __clz(stay);
+              over = stay != 0xffffffffu;
+              run += __shfl_sync(0xffffffffu, up, 31);
+            }
+            if (lane == 0) {
+              const int at = reinterpret_cast<int*>(bin_mass)[last];
+              edge_s.key = cand_key[at];
+              edge_s.index = cand_index[at];
+            }
+          }
+          __syncthreads();
+          if (tid > 0 && tid < ranks) {
+            cluster.map_shared_rank(&edge_s, tid)->key = edge_s.key;
+            cluster.map_shared_rank(&edge_s, tid)->index = edge_s.index;
+          }
+        }
+        cluster.sync();
+        edge_key = edge_s.key;
+        edge_index = edge_s.index;
+        if (kept_mass != nullptr) {
+          // exactly, in one order: what lies above the edge, and the edge's equals
+          double m = 0.0;
+          for (int i = tid; i < n; i += kSampleThreads) {
+            const float f = ToF32(v[i]);
+            const uint32_t key = KeyOf(f);
+            if (key > edge_key || (key == edge_key && lo + i <= edge_index)) m += weight(f);
+          }
+          *kept_mass = cluster_sum(m, red, told_mass);
+        }
+        return;
+      }
+    };
+    double mass = all;
+    if (by_k) {
+      const int b = find_bin([&](int c, float) { return c >= top_k; });
+      find_edge(b, true, top_k, 0.0, 0u, a.n, by_p ? &mass : nullptr);
+    }
+    if (by_p) {
+      const double share = fmax(static_cast<double>(top_p) * mass, 1e-300);  // above 0: the first one stays
+      const float rough = static_cast<float>(share);
+      const int last = by_k ? bin_of(ValueOf(edge_key)) : kBins - 1;
+      const int b = min(find_bin([&](int, float m) { return m >= rough; }), last);
+      double unused;
+      find_edge(b, false, 0, share, edge_key, edge_index, &unused);
+    }
+  }
+
+  // 4: what is kept, by warp, in index order.
+  const double least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
+  auto kept = [&](int i) -> double {  // the weight of a kept value, 0 of others
+    const float f = ToF32(v[i]);
+    const uint32_t key = KeyOf(f);
+    if (key < edge_key || (key == edge_key && lo + i > edge_index)) return 0.0;
+    const double w = weight(f);
+    return w < least ? 0.0 : w;
   };
   double mine = 0.0;
-  walk([&](int, double w) {
-    mine += w;
-    return false;
-  });
+  for (int i = w_lo + lane; i < w_hi; i += 32) mine += kept(i);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   __syncthreads();
-  if (lane == 0) red[warp] = mine;
+  if (lane == 0) warp_mass[warp] = mine;
   __syncthreads();
-  double total = 0.0;
-  int last = 0;  // the last warp that keeps any
-  for (int w = 0; w < kSampleWarps; ++w) {
-    total += red[w];
-    if (red[w] > 0.0) last = w;
-  }
-  const float u = __ldg(a.uniforms + row);
-  const double target = (u > 0.f ? fmin(static_cast<double>(u), 1.0) : 0.0) * total;
-  double sum = 0.0;
-  int chosen = last;
-  double in_front = 0.0;
-  for (int w = 0; w < kSampleWarps; ++w) {
-    if (red[w] > 0.0 && sum + red[w] > target) {
-      chosen = w;
-      in_front = sum;
-      break;
+  double part_mass = 0.0;
+#pragma unroll
+  for (int w = 0; w < kSampleWarps; ++w) part_mass += warp_mass[w];
+  double total = part_mass, in_front = 0.0;
+  int last_rank = 0, chosen_rank = 0;
+  if (ranks > 1) {
+    if (tid < ranks) *cluster.map_shared_rank(told_mass + rank, tid) = part_mass;
+    cluster.sync();
+    total = 0.0;
+    for (int q = 0; q < ranks; ++q) {
+      total += told_mass[q];
+      if (told_mass[q] > 0.0) last_rank = q;
     }
-    if (w == last) in_front = sum;
-    sum += red[w];
+  }
+  const double target = (u > 0.f ? fmin(static_cast<double>(u), 1.0) : 0.0) * total;
+  if (ranks > 1) {
+    chosen_rank = last_rank;
+    double run = 0.0;
+    for (int q = 0; q < ranks; ++q) {
+      if (q == last_rank) in_front = run;
+      if (told_mass[q] > 0.0 && run + told_mass[q] > target) {
+        chosen_rank = q;
+        in_front = run;
+        break;
+      }
+      run += told_mass[q];
+    }
+  }
+  if (rank != chosen_rank) return;
+  int chosen = 0;
+  {
+    double run = in_front, at_last = in_front;
+    bool found = false;
+    int last = 0;
+    for (int w = 0; w < kSampleWarps && !found; ++w) {
+      if (warp_mass[w] > 0.0) {
+        last = w;
+        at_last = run;
+        found = run + warp_mass[w] > target;
+      }
+      run += warp_mass[w];
+    }
+    chosen = last;
+    in_front = at_last;
   }
   if (warp != chosen) return;
   int token = -1;
   double run = in_front;
-  walk([&](int i, double w) {
-    double up = w;  // sums up to this lane
+  for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
+    const double w = i0 + lane < w_hi ? kept(i0 + lane) : 0.0;
+    const unsigned any = __ballot_sync(0xffffffffu, w > 0.0);
+    if (any == 0u) continue;
+    double up = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double t = __shfl_up_sync(0xffffffffu, up, o);
       if (lane >= o) up += t;
     }
-    const unsigned past = __ballot_sync(0xffffffffu, w > 0.0 && run + up > target), any = __ballot_sync(0xffffffffu, w > 0.0);
+    const unsigned past = __ballot_sync(0xffffffffu, w > 0.0 && run + up > target);
     if (past != 0u) {
-      token = i - lane + __ffs(past) - 1;
-      return true;
+      token = lo + i0 + __ffs(past) - 1;
+      break;
     }
-    if (any != 0u) token = i - lane + 31 - __clz(any);  // the last one kept, where roundings leave the target out of reach
+    token = lo + i0 + 31 - __clz(any);  // the last one kept, where roundings leave the target out of reach
     run += __shfl_sync(0xffffffffu, up, 31);
-    return false;
-  });
+  }
   if (lane == 0) a.out[row] = max(token, 0);
 }
+
+constexpr int kPartBytes = 160 * 1024;  // of a row that a CTA keeps
+
+cudaError_t PrepareSample()
+{
+  static OncePerDevice once;
+  return once.Run([](int) {
+    cudaError_t e = cudaFuncSetAttribute(SampleKernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPartBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(SampleKernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPartBytes);
+    return e;
+  });
+}
+KernelSetup g_setup(PrepareSample, nullptr);
 
 }  // namespace
 }  // namespace tlaloc_b200
@@ -239,10 +618,24 @@ extern "C" int tlaloc_b200_sample(const void* logits, int64_t ld, int32_t dtype,
   if (!IsFloatType(dtype)) return Fail(kInvalid, "%s: logits must be f32 or bf16", op);
   if (rows < 0 || n < 1 || ld < n) return Fail(kInvalid, "%s: bad sizes", op);
   if (rows == 0) return kOk;
-  const SampleArgs a = {logits, ld, uniforms, temperature, top_k, top_p, min_p, temperature_all, top_p_all, min_p_all, top_k_all, out, n};
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == TLALOC_B200_F32 ? LaunchChained(SampleKernel<float>, rows, kSampleThreads, 0, st, a)
-                                                 : LaunchChained(SampleKernel<__nv_bfloat16>, rows, kSampleThreads, 0, st, a);
+  cudaError_t e = PrepareSample();
+  if (e != cudaSuccess) return CudaFail("SAMPLE set-up", e);
+  // A CTA takes 16384 values, 64 KB of f32: three of them fit an SM, and few rows of a large vocabulary still spread over eight.
+  int ranks = 1;
+  while (ranks < kMaxRanks && static_cast<long long>(ranks) * 16384 < n) ranks *= 2;
+  SampleArgs a = {logits, ld, uniforms, temperature, top_k, top_p, min_p, temperature_all, top_p_all, min_p_all, top_k_all, out, n, 0, 0};
+  a.per = ((n + ranks - 1) / ranks + 7) / 8 * 8;
+  const size_t bytes = static_cast<size_t>(a.per) * DtypeBytes(dtype);
+  a.on_chip = bytes <= kPartBytes ? 1 : 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(rows, ranks);
+  cfg.blockDim = dim3(kSampleThreads);
+  cfg.dynamicSmemBytes = a.on_chip ? (bytes + 15) / 16 * 16 : 0;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attrs[2];
+  cfg.numAttrs = ChainAttributes(attrs, ranks);
+  cfg.attrs = attrs;
+  e = dtype == TLALOC_B200_F32 ? cudaLaunchKernelEx(&cfg, SampleKernel<float>, a) : cudaLaunchKernelEx(&cfg, SampleKernel<__nv_bfloat16>, a);
   if (e != cudaSuccess) return CudaFail("SAMPLE launch", e);
   CountLaunches(1);
   return kOk;
