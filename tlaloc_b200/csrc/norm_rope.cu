@@ -101,9 +101,155 @@ __global__ void __launch_bounds__(32 * kPlainWarps) NormRopePlain(const __grid_c
   }
 }
 
+// Heads, rotated parts' halves and strides of whole 16-byte words.  L lanes share a head, eight channels each; a warp takes 32 / L head slots of one token at a time, and U
+// such groups with all their loads in flight before the first sum.  A lane's place in the head is the same in every group, so cosines and sines are read once a warp.  The
+// partner of channel j of the first half lies rot / 16 lanes further on; pairs (2i, 2i + 1) lie in one lane.
+__device__ __forceinline__ void LoadRaw(const float* p, uint4 (&raw)[2])
+{
+  raw[0] = __ldcg(reinterpret_cast<const uint4*>(p));
+  raw[1] = __ldcg(reinterpret_cast<const uint4*>(p) + 1);
+}
+__device__ __forceinline__ void LoadRaw(const __nv_bfloat16* p, uint4 (&raw)[1]) { raw[0] = __ldcg(reinterpret_cast<const uint4*>(p)); }
+__device__ __forceinline__ void Widen(const uint4 (&raw)[2], float (&v)[8])
+{
+  v[0] = __uint_as_float(raw[0].x), v[1] = __uint_as_float(raw[0].y), v[2] = __uint_as_float(raw[0].z), v[3] = __uint_as_float(raw[0].w);
+  v[4] = __uint_as_float(raw[1].x), v[5] = __uint_as_float(raw[1].y), v[6] = __uint_as_float(raw[1].z), v[7] = __uint_as_float(raw[1].w);
+}
+__device__ __forceinline__ void Widen(const uint4 (&raw)[1], float (&v)[8])
+{
+  const uint32_t w[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void Store8(float* p, const float (&v)[8])
+{
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void Store8(__nv_bfloat16* p, const float (&v)[8])
+{
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void Store8(__nv_fp8_e4m3* p, const float (&v)[8])
+{
+  uint32_t w[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+    w[i >> 1] |= two << (16 * (i & 1));
+  }
+  *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+}
+
+constexpr int kFastWarps = 8;
+template <typename XT, typename QT, typename KVT, int L, int U>
+__global__ void __launch_bounds__(32 * kFastWarps) NormRopeFast(const __grid_constant__ NormRopeArgs a)
+{
+  constexpr int kGroups = 32 / L;  // head slots of a warp at a time
+  GridDependencySync();
+  const int t = blockIdx.x, lane = threadIdx.x & 31, at = lane % L, c = at * 8;  // this lane's channels [c, c + 8)
+  const int slots = a.H + 2 * a.Hkv, h0 = (blockIdx.y * kFastWarps + (threadIdx.x >> 5)) * (kGroups * U) + lane / L;
+  const int slot = __ldg(a.slots + t), pos = min(max(__ldg(a.positions + t), 0), a.max_pos - 1), half = a.rot >> 1;
+  const bool mine = c < a.D;
+  uint4 raw[U][sizeof(XT) / 2];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int h = h0 + u * kGroups;
+    if (h < slots && mine) {
+      const HeadSlot<XT, QT, KVT> s(a, t, h, slot);
+      LoadRaw(s.src + c, raw[u]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < static_cast<int>(sizeof(XT) / 2); ++e) raw[u][e] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  // cos and, with the sign of the partner's term, sin of this lane's channels: 1 and 0 behind the rotated part.
+  float cs[8], sn[8];
+  const float* cos_p = a.cos_t + static_cast<int64_t>(pos) * half;
+  const float* sin_p = a.sin_t + static_cast<int64_t>(pos) * half;
+  const bool second = c >= half;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int j = c + e;
+    const bool in = j < a.rot;
+    const int i = a.interleaved ? j >> 1 : (second ? j - half : j);
+    cs[e] = in ? __ldg(cos_p + i) : 1.f;
+    sn[e] = in ? __ldg(sin_p + i) : 0.f;
+    if (a.interleaved ? (e & 1) == 0 : !second) sn[e] = -sn[e];
+  }
+  const int partner = a.interleaved ? lane : (c < half ? lane + half / 8 : c < a.rot ? lane - half / 8 : lane);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int h = h0 + u * kGroups;
+    const bool there = h < slots;
+    const HeadSlot<XT, QT, KVT> s(a, t, there ? h : 0, slot);
+    float v[8];
+    Widen(raw[u], v);
+    const float* gain = there ? s.gain : nullptr;
+    if (a.q_gain != nullptr) {  // the same for every lane of the grid: values, which are not normed, go along
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (gain != nullptr && mine) {
+        const float rsq = __frsqrt_rn(__fadd_rn(__fdiv_rn(sum, static_cast<float>(a.D)), a.eps));
+        const float4 g0 = __ldg(reinterpret_cast<const float4*>(gain + c)), g1 = __ldg(reinterpret_cast<const float4*>(gain + c) + 1);
+        const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __fmul_rn(__fmul_rn(v[e], rsq), g[e]);
+      }
+    }
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = a.interleaved ? v[e ^ 1] : __shfl_sync(0xffffffffu, v[e], partner);
+    if (there && s.rotate) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c + e < a.rot) v[e] = __fadd_rn(__fmul_rn(v[e], cs[e]), __fmul_rn(w[e], sn[e]));
+    }
+    if (there && mine) {
+      if (s.q_dst != nullptr) Store8(s.q_dst + c, v);
+      else if (s.kv_dst != nullptr) Store8(s.kv_dst + c, v);
+    }
+  }
+}
+
+// Whole words everywhere: heads of multiples of 8 channels up to 256, halves of the rotated part too (pairs beside one another need none), addresses and strides of 16 bytes.
+bool FastApplies(const NormRopeArgs& a, size_t x_bytes)
+{
+  auto words = [&](int64_t ld) { return ld * x_bytes % 16 == 0; };
+  return !a.faithful && a.D % 8 == 0 && a.D <= 256 && (a.interleaved || a.rot % 16 == 0) && Aligned16(a.q) && Aligned16(a.k) && Aligned16(a.v) && words(a.ld_q) &&
+         words(a.ld_k) && words(a.ld_v) && Aligned16(a.q_out) && Aligned16(a.kc) && Aligned16(a.vc) && Aligned16(a.q_gain) && Aligned16(a.k_gain);
+}
+
+template <typename XT, typename QT, typename KVT, int L>
+cudaError_t LaunchFast(const NormRopeArgs& a, cudaStream_t st)
+{
+  // Four groups of heads a warp while that leaves every SM sixteen warps; few tokens are bound by latency and take one.
+  const int slots = a.H + 2 * a.Hkv, per_warp = 32 / L;
+  if (static_cast<long long>(a.T) * slots / (4 * per_warp) >= 148 * 16) {
+    return LaunchChained(NormRopeFast<XT, QT, KVT, L, 4>, dim3(a.T, (slots + 4 * per_warp * kFastWarps - 1) / (4 * per_warp * kFastWarps)), 32 * kFastWarps, 0, st, a);
+  }
+  return LaunchChained(NormRopeFast<XT, QT, KVT, L, 1>, dim3(a.T, (slots + per_warp * kFastWarps - 1) / (per_warp * kFastWarps)), 32 * kFastWarps, 0, st, a);
+}
+
 template <typename XT, typename QT, typename KVT>
 cudaError_t LaunchNormRope(const NormRopeArgs& a, cudaStream_t st)
 {
+  if (FastApplies(a, sizeof(XT))) {
+    if (a.D <= 64) return LaunchFast<XT, QT, KVT, 8>(a, st);
+    return a.D <= 128 ? LaunchFast<XT, QT, KVT, 16>(a, st) : LaunchFast<XT, QT, KVT, 32>(a, st);
+  }
   const dim3 grid(a.T, (a.H + 2 * a.Hkv + kPlainWarps - 1) / kPlainWarps);
   return LaunchChained(NormRopePlain<XT, QT, KVT>, grid, 32 * kPlainWarps, 0, st, a);
 }

@@ -10,11 +10,14 @@
 //
 // A cluster of CTAs shares a row; each reads its part once and keeps it in shared memory where it fits.  Passes over the part:
 //   1  the largest value
-//   2  (with top-k or top-p) how many values, and roughly which mass, lie in each of 1024 bins of (max - x) / T, and the exact mass of all
-//   3  per edge: the exact count and mass above the bin that it lies in; the bin's values go to one CTA, which ranks them and finds the edge.  The rough masses of
-//      pass 2 only say where to look: the exact ones decide, and move on to a neighbouring bin if they must.  A bin with more values than a CTA holds is halved by
-//      value, over and over (equal logits by the thousand)
-//   4  the mass that is kept, by warp, and then the draw, in the one warp whose stretch it falls into
+//   2  (with top-k or top-p) how many values, and roughly which mass, lie in each of 1024 bins of (max - x) / T, and for top-p the exact mass of all
+//   3  where the bins from the largest value down to the edge hold no more than 512 values, as they mostly do: these go to one CTA, which ranks them, a thread each, and
+//      finds both edges and the token among them
+//   Otherwise, per edge: the exact count and mass above the bin that it lies in; the bin's values go to one CTA, which ranks them and finds the edge.  The rough masses
+//      of pass 2 only say where to look: the exact ones decide, and move on to a neighbouring bin if they must.  A bin with more values than a CTA ranks is halved by
+//      value, over and over (equal logits by the thousand).  Then
+//   4  the mass that is kept, by warp, and the draw, in the one warp whose stretch it falls into
+// Without top-k and top-p there are passes 1 and 4 alone, which the f64 units bound: nine operations an exponential.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -76,13 +79,14 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
   extern __shared__ __align__(16) unsigned char part_raw[];  // this CTA's part of the row, where it fits
   __shared__ double table[kExpTable];
   __shared__ double red[kSampleWarps], told_mass[kMaxRanks], warp_mass[kSampleWarps];
-  __shared__ int ired[kSampleWarps], told_count[kMaxRanks];
-  __shared__ uint32_t kred[kSampleWarps], told_key[kMaxRanks];
+  __shared__ double told_masses[2][kMaxRanks];
+  __shared__ int ired[kSampleWarps], told_count[kMaxRanks], told_counts[2][kMaxRanks];
+  __shared__ uint32_t kred[kSampleWarps], told_key[kMaxRanks], range_s[2];
   __shared__ int bin_count[kBins];
-  __shared__ float bin_mass[kBins];
+  __shared__ __align__(16) float bin_mass[kBins];
   __shared__ uint32_t cand_key[kRanked];
   __shared__ int cand_index[kRanked];
-  __shared__ int cand_n;
+  __shared__ int cand_n, cand_token, cand_last, cand_done;
   __shared__ struct {
     uint32_t key;
     int index;
@@ -165,7 +169,7 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
     for (int q = 0; q < ranks; ++q) best = max(best, told_key[q]);
   }
   const float top = ValueOf(best);
-  const int chunk = ((n + kSampleWarps - 1) / kSampleWarps + 31) / 32 * 32;  // a warp's stretch of the part
+  const int chunk = ((n + kSampleWarps - 1) / kSampleWarps + 31) / 32 * 32;  // a warp's stretch of the part: whole 16-byte words
   const int w_lo = min(warp * chunk, n), w_hi = min(w_lo + chunk, n);
 
   if (!(temperature > 0.f) || top == -INFINITY) {  // greedy, or nothing to draw: the first of the largest, index 0 of a row without one
@@ -188,10 +192,33 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
   }
 
   const double scale = 1.4426950408889634074 / static_cast<double>(temperature), dtop = static_cast<double>(top);
-  auto weight = [&](float f) -> double {
-    if (f == top) return 1.0;
-    if (!(f > -INFINITY) || top == INFINITY) return 0.0;
+  const bool infinite = top == INFINITY;
+  auto weight = [&](float f) -> double {  // 1 for the largest: 2^0 is exact
+    if (infinite) return f == INFINITY ? 1.0 : 0.0;
+    if (!(f == f)) return 0.0;
     return TableExp2((static_cast<double>(f) - dtop) * scale, table);
+  };
+  // A lane's values [i, i + kVec) of the part, -infinity behind its end.
+  constexpr int kVec = 16 / static_cast<int>(sizeof(XT));
+  auto values = [&](int i, int end, float (&f)[kVec]) {
+    if (a.on_chip) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(part + i);  // the part's end is padded to whole words
+      const XT* e = reinterpret_cast<const XT*>(&raw);
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) f[k] = i + k < end ? ToF32(e[k]) : -INFINITY;
+    } else {
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) f[k] = i + k < end ? ToF32(x[i + k]) : -INFINITY;
+    }
+  };
+  auto each = [&](auto&& work) {  // work(place in the part, value), every place of it
+    for (int i = tid * kVec; i < n; i += kSampleThreads * kVec) {
+      float f[kVec];
+      values(i, n, f);
+#pragma unroll
+      for (int k = 0; k < kVec; ++k)
+        if (i + k < n) work(i + k, f[k]);
+    }
   };
   // The bin of a value: a function that does not rise with it, however it is rounded.
   const float fscale = fminf(static_cast<float>(scale) * kBinsPerOctave, 3.0e38f);
@@ -213,8 +240,7 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
     }
     __syncthreads();
     double all = 0.0;
-    for (int i = tid; i < n; i += kSampleThreads) {
-      const float f = ToF32(v[i]);
+    each([&](int, float f) {
       const int b = bin_of(f);
       atomicAdd(&bin_count[b], 1);
       if (by_p) {
@@ -222,10 +248,11 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
         all += w;
         atomicAdd(&bin_mass[b], static_cast<float>(w));
       }
-    }
+    });
     if (by_p) all = cluster_sum(all, red, told_mass);
-    else __syncthreads();
-    if (ranks > 1) {  // the row's bins: every rank adds up an equal share of them over all ranks and tells everyone
+    auto add_bins = [&]() {  // the row's bins: every rank adds up an equal share of them over all ranks and tells everyone
+      __syncthreads();
+      if (ranks == 1) return;
       cluster.sync();
       const int share = kBins / ranks, b = rank * share + tid;
       int c = 0;
@@ -244,10 +271,12 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
         }
       }
       cluster.sync();
-    }
-    // The first bin at whose end `enough(count, mass)` holds; the last one if it never does.
-    auto find_bin = [&](auto&& enough) {
-      __shared__ int found_s;
+    };
+    add_bins();
+    bool redo = false;
+    // The first bin at whose end `enough(count, mass)` holds, the last one if it never does; *upto: the count there.
+    auto find_bin = [&](auto&& enough, int* upto) {
+      __shared__ int found_s, upto_s;
       __shared__ int cs[kSampleWarps];
       __shared__ float ms[kSampleWarps];
       constexpr int kEach = kBins / kSampleThreads;
@@ -291,11 +320,156 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
         if (enough(cb + c[e], mb + m[e])) atomicMin(&found_s, tid * kEach + e);
       __syncthreads();
       const int b = found_s;
+      if (tid == b / kEach) upto_s = cb + (b % kEach == 0 ? c[0] : c[kEach - 1]);
+      __syncthreads();
+      if (upto != nullptr) *upto = upto_s;
       __syncthreads();
       return b;
     };
+    static_assert(kBins / kSampleThreads == 2, "find_bin: two bins a thread");
 
-    // 3: the edge in or next to bin `b`.  Counting: the value of rank `want_count`.  Otherwise: the last value whose betters hold less than `want_mass`, none beyond
+    // Everything down to the edge in rank 0, if that is few enough.
+    const double least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
+    {
+      int few = 0;
+      const float rough = static_cast<float>(static_cast<double>(top_p) * all) * 1.001f;
+      const int b = by_k ? find_bin([&](int c, float) { return c >= top_k; }, &few) : find_bin([&](int, float m) { return m >= rough; }, &few);
+      if (few <= kRanked) {
+        if (tid == 0) cand_n = 0;
+        cluster.sync();
+        int* const count0 = cluster.map_shared_rank(&cand_n, 0);
+        uint32_t* const key0 = cluster.map_shared_rank(cand_key, 0);
+        int* const index0 = cluster.map_shared_rank(cand_index, 0);
+        each([&](int i, float f) {
+          if (bin_of(f) > b) return;
+          const int at = atomicAdd(count0, 1);
+          key0[at] = KeyOf(f);
+          index0[at] = lo + i;
+        });
+        cluster.sync();
+        if (rank == 0) {
+          // By rank, in the bins' place: index, then weight.
+          int* const s_index = bin_count;
+          double* const s_weight = reinterpret_cast<double*>(bin_mass);
+          static_assert(sizeof(bin_mass) >= sizeof(double) * kRanked && kRanked == kSampleThreads, "a thread a value");
+          const int m = cand_n;
+          if (tid < m) {
+            const uint32_t key = cand_key[tid];
+            const int index = cand_index[tid];
+            int better = 0;
+            for (int j = 0; j < m; ++j) better += cand_key[j] > key || (cand_key[j] == key && cand_index[j] < index) ? 1 : 0;
+            s_index[better] = index;
+            s_weight[better] = weight(ValueOf(key));
+          }
+          if (tid == 0) cand_token = 0x7fffffff, cand_last = 0;
+          __syncthreads();
+          const double w = tid < m ? s_weight[tid] : 0.0;
+          double up = w;  // sums up to this rank
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const double t = __shfl_up_sync(0xffffffffu, up, o);
+            if (lane >= o) up += t;
+          }
+          double front = __shfl_up_sync(0xffffffffu, up, 1);
+          if (lane == 0) front = 0.0;
+          if (lane == 31) red[warp] = up;
+          __syncthreads();
+          double run = 0.0, in_all = 0.0;
+          for (int q = 0; q < kSampleWarps; ++q) {
+            if (q < warp) run += red[q];
+            in_all += red[q];
+          }
+          front += run;
+          if (by_k && tid == min(top_k, m) - 1) warp_mass[0] = run + up;
+          __syncthreads();
+          const double share = by_p ? fmax(static_cast<double>(top_p) * (by_k ? warp_mass[0] : all), 1e-300) : 0.0;
+          const bool reached = by_k || in_all >= share || m == a.n;  // the rough masses may have stopped short
+          const bool keep = tid < m && (!by_k || tid < top_k) && (!by_p || front < share || tid == 0) && w >= least && w > 0.0;
+          const int index = tid < m ? s_index[tid] : 0;
+          __syncthreads();
+          if (tid < m) s_weight[tid] = keep ? w : 0.0;
+          const double kept_all = block_sum(keep ? w : 0.0, red);
+          const double target = (u > 0.f ? fmin(static_cast<double>(u), 1.0) : 0.0) * kept_all;
+          if (keep) {
+            double before = 0.0;  // what is kept at lower indices
+            for (int j = 0; j < m; ++j)
+              if (s_index[j] < index) before += s_weight[j];
+            if (before + w > target) atomicMin(&cand_token, index);
+            atomicMax(&cand_last, index);
+          }
+          __syncthreads();
+          if (tid == 0 && reached) a.out[row] = cand_token != 0x7fffffff ? cand_token : cand_last;  // the last one kept, where roundings leave the target out of reach
+          if (tid < ranks) *cluster.map_shared_rank(&cand_done, tid) = reached ? 1 : 0;
+        }
+        cluster.sync();
+        if (cand_done != 0) return;
+        // The bins are gone where they were ranked: take them from a rank that has them (there is one, or they are counted again).
+        redo = true;
+      }
+    }
+    if (redo) {
+      cluster.sync();
+      for (int i = tid; i < kBins; i += kSampleThreads) {
+        bin_count[i] = 0;
+        bin_mass[i] = 0.f;
+      }
+      __syncthreads();
+      each([&](int, float f) {
+        const int b = bin_of(f);
+        atomicAdd(&bin_count[b], 1);
+        atomicAdd(&bin_mass[b], static_cast<float>(weight(f)));
+      });
+      add_bins();
+    }
+
+    auto mass_upto_edge = [&]() {
+      double m = 0.0;
+      each([&](int i, float f) {
+        const uint32_t key = KeyOf(f);
+        if (key > edge_key || (key == edge_key && lo + i <= edge_index)) m += weight(f);
+      });
+      return cluster_sum(m, red, told_mass);
+    };
+    // Four sums at once.
+    auto cluster_sums = [&](int& c0, int& c1, double& m0, double& m1) {
+      c0 = block_sum(c0, ired);
+      c1 = block_sum(c1, ired);
+      m0 = block_sum(m0, red);
+      m1 = block_sum(m1, red);
+      if (ranks == 1) return;
+      if (tid < ranks) {
+        *cluster.map_shared_rank(told_counts[0] + rank, tid) = c0;
+        *cluster.map_shared_rank(told_counts[1] + rank, tid) = c1;
+        *cluster.map_shared_rank(told_masses[0] + rank, tid) = m0;
+        *cluster.map_shared_rank(told_masses[1] + rank, tid) = m1;
+      }
+      cluster.sync();
+      c0 = c1 = 0;
+      m0 = m1 = 0.0;
+      for (int q = 0; q < ranks; ++q) {
+        c0 += told_counts[0][q];
+        c1 += told_counts[1][q];
+        m0 += told_masses[0][q];
+        m1 += told_masses[1][q];
+      }
+      cluster.sync();
+    };
+    // The range over all ranks; cluster_sums, which follows it, parts this one's words from the next one's.
+    auto cluster_range = [&](uint32_t& least_key, uint32_t& most_key) {
+      least_key = __reduce_min_sync(0xffffffffu, least_key);
+      most_key = __reduce_max_sync(0xffffffffu, most_key);
+      if (tid == 0) range_s[0] = 0xffffffffu, range_s[1] = 0u;
+      cluster.sync();
+      if (lane < ranks) {
+        atomicMin(cluster.map_shared_rank(&range_s[0], lane), least_key);
+        atomicMax(cluster.map_shared_rank(&range_s[1], lane), most_key);
+      }
+      cluster.sync();
+      least_key = range_s[0];
+      most_key = range_s[1];
+      __syncthreads();
+    };
+    // The edge in or next to bin `b`.  Counting: the value of rank `want_count`.  Otherwise: the last value whose betters hold less than `want_mass`, none beyond
     // (limit_key, limit_index).  kept_mass, if given: the exact mass of what is kept.
     auto find_edge = [&](int b, bool counting, int want_count, double want_mass, uint32_t limit_key, int limit_index, double* kept_mass) {
       int moved = 0;  // which way: never back, whatever sums of the same values in two groupings say
@@ -303,25 +477,25 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
         // Exactly what lies above the bin, and in it.
         int above_n = 0, in_n = 0;
         double above = 0.0, in = 0.0;
-        for (int i = tid; i < n; i += kSampleThreads) {
-          const float f = ToF32(v[i]);
+        uint32_t k_lo = 0xffffffffu, k_hi = 0;  // the bin's values lie between these keys
+        each([&](int i, float f) {
           const int at = bin_of(f);
-          if (at > b) continue;
+          if (at > b) return;
           const uint32_t key = KeyOf(f);
-          if (key < limit_key || (key == limit_key && lo + i > limit_index)) continue;
-          const double w = weight(f);
+          if (key < limit_key || (key == limit_key && lo + i > limit_index)) return;
+          const double w = counting ? 0.0 : weight(f);
           if (at < b) {
             ++above_n;
             above += w;
           } else {
             ++in_n;
             in += w;
+            k_lo = min(k_lo, key);
+            k_hi = max(k_hi, key);
           }
-        }
-        above_n = cluster_sum(above_n, ired, told_count);
-        in_n = cluster_sum(in_n, ired, told_count);
-        above = cluster_sum(above, red, told_mass);
-        in = cluster_sum(in, red, told_mass);
+        });
+        cluster_range(k_lo, k_hi);
+        cluster_sums(above_n, in_n, above, in);
         if (!counting && above_n > 0 && above >= want_mass) {  // roundings of the rough masses: the edge lies higher
           if (moved <= 0) {
             moved = -1;
@@ -336,21 +510,20 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
           continue;
         }
         if (in_n == 0) return;  // all of them stay
-        // The bin's values between these keys, while they are too many for one CTA: halved by value.
-        uint32_t k_lo = 0, k_hi = 0xffffffffu;
+        // While they are too many for one CTA: halved by value.
         while (in_n > kRanked && k_lo < k_hi) {
           const uint32_t mid = k_lo + (k_hi - k_lo) / 2;  // the upper half: keys above it
           int up_n = 0;
           double up = 0.0;
-          for (int i = tid; i < n; i += kSampleThreads) {
-            const float f = ToF32(v[i]);
+          each([&](int i, float f) {
             const uint32_t key = KeyOf(f);
-            if (key <= mid || key > k_hi || bin_of(f) != b || key < limit_key || (key == limit_key && lo + i > limit_index)) continue;
+            if (key <= mid || key > k_hi || bin_of(f) != b || key < limit_key || (key == limit_key && lo + i > limit_index)) return;
             ++up_n;
-            up += weight(f);
-          }
-          up_n = cluster_sum(up_n, ired, told_count);
-          up = cluster_sum(up, red, told_mass);
+            if (!counting) up += weight(f);
+          });
+          int none_n = 0;
+          double none = 0.0;
+          cluster_sums(up_n, none_n, up, none);
           // Neither half is taken empty.
           const bool higher = up_n > 0 && (up_n == in_n || (counting ? above_n + up_n >= want_count : above + up >= want_mass));
           if (higher) {
@@ -407,8 +580,8 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
           cluster.sync();
           edge_key = key;
           edge_index = edge_s.index;
-          if (kept_mass != nullptr) *kept_mass = above + quota * w;
           cluster.sync();
+          if (kept_mass != nullptr) *kept_mass = mass_upto_edge();
           return;
         }
         // The values of the bin (or of what is left of it) in rank 0, in any order.
@@ -417,14 +590,13 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
         int* const count0 = cluster.map_shared_rank(&cand_n, 0);
         uint32_t* const key0 = cluster.map_shared_rank(cand_key, 0);
         int* const index0 = cluster.map_shared_rank(cand_index, 0);
-        for (int i = tid; i < n; i += kSampleThreads) {
-          const float f = ToF32(v[i]);
+        each([&](int i, float f) {
           const uint32_t key = KeyOf(f);
-          if (bin_of(f) != b || key < k_lo || key > k_hi || key < limit_key || (key == limit_key && lo + i > limit_index)) continue;
+          if (bin_of(f) != b || key < k_lo || key > k_hi || key < limit_key || (key == limit_key && lo + i > limit_index)) return;
           const int at = atomicAdd(count0, 1);
           key0[at] = key;
           index0[at] = lo + i;
-        }
+        });
         cluster.sync();
         if (rank == 0) {
           // Each value's betters among them, their number and mass: the edge is the one whose betters leave room and which itself takes the last of it.
@@ -479,28 +651,21 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
         edge_key = edge_s.key;
         edge_index = edge_s.index;
         if (kept_mass != nullptr) {
-          // exactly, in one order: what lies above the edge, and the edge's equals
-          double m = 0.0;
-          for (int i = tid; i < n; i += kSampleThreads) {
-            const float f = ToF32(v[i]);
-            const uint32_t key = KeyOf(f);
-            if (key > edge_key || (key == edge_key && lo + i <= edge_index)) m += weight(f);
-          }
-          *kept_mass = cluster_sum(m, red, told_mass);
+          *kept_mass = mass_upto_edge();
         }
         return;
       }
     };
     double mass = all;
     if (by_k) {
-      const int b = find_bin([&](int c, float) { return c >= top_k; });
+      const int b = find_bin([&](int c, float) { return c >= top_k; }, nullptr);
       find_edge(b, true, top_k, 0.0, 0u, a.n, by_p ? &mass : nullptr);
     }
     if (by_p) {
       const double share = fmax(static_cast<double>(top_p) * mass, 1e-300);  // above 0: the first one stays
       const float rough = static_cast<float>(share);
       const int last = by_k ? bin_of(ValueOf(edge_key)) : kBins - 1;
-      const int b = min(find_bin([&](int, float m) { return m >= rough; }), last);
+      const int b = min(find_bin([&](int, float m) { return m >= rough; }, nullptr), last);
       double unused;
       find_edge(b, false, 0, share, edge_key, edge_index, &unused);
     }
@@ -508,15 +673,22 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
 
   // 4: what is kept, by warp, in index order.
   const double least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
-  auto kept = [&](int i) -> double {  // the weight of a kept value, 0 of others
-    const float f = ToF32(v[i]);
-    const uint32_t key = KeyOf(f);
-    if (key < edge_key || (key == edge_key && lo + i > edge_index)) return 0.0;
+  const bool whole = edge_key == 0u;
+  auto kept = [&](int i, float f) -> double {  // the weight of a kept value, 0 of others
+    if (!whole) {
+      const uint32_t key = KeyOf(f);
+      if (key < edge_key || (key == edge_key && lo + i > edge_index)) return 0.0;
+    }
     const double w = weight(f);
     return w < least ? 0.0 : w;
   };
   double mine = 0.0;
-  for (int i = w_lo + lane; i < w_hi; i += 32) mine += kept(i);
+  for (int i = w_lo + lane * kVec; i < w_hi; i += 32 * kVec) {
+    float f[kVec];
+    values(i, w_hi, f);
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) mine += kept(i + k, f[k]);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   __syncthreads();
@@ -570,22 +742,41 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
   if (warp != chosen) return;
   int token = -1;
   double run = in_front;
-  for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
-    const double w = i0 + lane < w_hi ? kept(i0 + lane) : 0.0;
-    const unsigned any = __ballot_sync(0xffffffffu, w > 0.0);
+  for (int i0 = w_lo; i0 < w_hi; i0 += 32 * kVec) {
+    const int i = i0 + lane * kVec;
+    float f[kVec];
+    double w[kVec], sum = 0.0;
+    if (i < w_hi) values(i, w_hi, f);
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      w[k] = i + k < w_hi ? kept(i + k, f[k]) : 0.0;
+      sum += w[k];
+    }
+    const unsigned any = __ballot_sync(0xffffffffu, sum > 0.0);
     if (any == 0u) continue;
-    double up = w;
+    double up = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double t = __shfl_up_sync(0xffffffffu, up, o);
       if (lane >= o) up += t;
     }
-    const unsigned past = __ballot_sync(0xffffffffu, w > 0.0 && run + up > target);
-    if (past != 0u) {
-      token = lo + i0 + __ffs(past) - 1;
-      break;
+    double front = __shfl_up_sync(0xffffffffu, up, 1);
+    if (lane == 0) front = 0.0;
+    const unsigned past = __ballot_sync(0xffffffffu, sum > 0.0 && run + up > target);
+    const int who = past != 0u ? __ffs(past) - 1 : 31 - __clz(any);  // the last one that keeps any, where roundings leave the target out of reach
+    int here = -1;
+    bool over = false;
+    double at = run + front;
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      at += w[k];
+      if (w[k] > 0.0 && !over) {
+        here = lo + i + k;
+        over = past != 0u && at > target;
+      }
     }
-    token = lo + i0 + 31 - __clz(any);  // the last one kept, where roundings leave the target out of reach
+    token = __shfl_sync(0xffffffffu, here, who);
+    if (past != 0u) break;
     run += __shfl_sync(0xffffffffu, up, 31);
   }
   if (lane == 0) a.out[row] = max(token, 0);
