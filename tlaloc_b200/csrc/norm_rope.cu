@@ -150,85 +150,118 @@ __device__ __forceinline__ void Store8(__nv_fp8_e4m3* p, const float (&v)[8])
   *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
 }
 
+// Four words of a table.
+__device__ __forceinline__ void Load4(const float* p, float* v)
+{
+  const float4 x = __ldg(reinterpret_cast<const float4*>(p));
+  v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+}
+
 constexpr int kFastWarps = 8;
 template <typename XT, typename QT, typename KVT, int L, int U>
-__global__ void __launch_bounds__(32 * kFastWarps) NormRopeFast(const __grid_constant__ NormRopeArgs a)
+__global__ void __launch_bounds__(32 * kFastWarps) NormRopeFast(const __grid_constant__ NormRopeArgs a, const int chunks, const float inv_d)
 {
   constexpr int kGroups = 32 / L;  // head slots of a warp at a time
   GridDependencySync();
-  const int t = blockIdx.x, lane = threadIdx.x & 31, at = lane % L, c = at * 8;  // this lane's channels [c, c + 8)
-  const int slots = a.H + 2 * a.Hkv, h0 = (blockIdx.y * kFastWarps + (threadIdx.x >> 5)) * (kGroups * U) + lane / L;
+  const unsigned id = blockIdx.x * kFastWarps + (threadIdx.x >> 5);
+  const int t = static_cast<int>(id / chunks), lane = threadIdx.x & 31, c = lane % L * 8;  // this lane's channels [c, c + 8)
+  if (t >= a.T) return;
+  const int h0 = static_cast<int>(id - t * chunks) * (kGroups * U) + lane / L;
   const int slot = __ldg(a.slots + t), pos = min(max(__ldg(a.positions + t), 0), a.max_pos - 1), half = a.rot >> 1;
-  const bool mine = c < a.D;
+  const bool mine = c < a.D, in = c < a.rot, written = slot >= 0 && slot < a.num_slots;
+  const XT* const q = static_cast<const XT*>(a.q) + t * a.ld_q;
+  const XT* const k = static_cast<const XT*>(a.k) + t * a.ld_k;
+  const XT* const v_rows = static_cast<const XT*>(a.v) + t * a.ld_v;
   uint4 raw[U][sizeof(XT) / 2];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int h = h0 + u * kGroups;
-    if (h < slots && mine) {
-      const HeadSlot<XT, QT, KVT> s(a, t, h, slot);
-      LoadRaw(s.src + c, raw[u]);
-    } else {
 #pragma unroll
-      for (int e = 0; e < static_cast<int>(sizeof(XT) / 2); ++e) raw[u][e] = make_uint4(0u, 0u, 0u, 0u);
+    for (int e = 0; e < static_cast<int>(sizeof(XT) / 2); ++e) raw[u][e] = make_uint4(0u, 0u, 0u, 0u);
+    if (h < a.H + 2 * a.Hkv && mine) {
+      const XT* const row = h < a.H ? q : h < a.H + a.Hkv ? k : v_rows;
+      LoadRaw(row + (h < a.H ? h : h < a.H + a.Hkv ? h - a.H : h - a.H - a.Hkv) * a.D + c, raw[u]);
     }
   }
-  // cos and, with the sign of the partner's term, sin of this lane's channels: 1 and 0 behind the rotated part.
+  // cos and, with the sign of the partner's term, sin of this lane's channels.
   float cs[8], sn[8];
-  const float* cos_p = a.cos_t + static_cast<int64_t>(pos) * half;
-  const float* sin_p = a.sin_t + static_cast<int64_t>(pos) * half;
-  const bool second = c >= half;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int j = c + e;
-    const bool in = j < a.rot;
-    const int i = a.interleaved ? j >> 1 : (second ? j - half : j);
-    cs[e] = in ? __ldg(cos_p + i) : 1.f;
-    sn[e] = in ? __ldg(sin_p + i) : 0.f;
-    if (a.interleaved ? (e & 1) == 0 : !second) sn[e] = -sn[e];
+  for (int e = 0; e < 8; ++e) cs[e] = 1.f, sn[e] = 0.f;
+  const bool second = c >= half;
+  if (in) {
+    const float* const cos_p = a.cos_t + static_cast<int64_t>(pos) * half;
+    const float* const sin_p = a.sin_t + static_cast<int64_t>(pos) * half;
+    if (a.interleaved) {
+      float x[4], y[4];
+      Load4(cos_p + (c >> 1), x);
+      Load4(sin_p + (c >> 1), y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) cs[e] = x[e >> 1], sn[e] = (e & 1) == 0 ? -y[e >> 1] : y[e >> 1];
+    } else {
+      const int i = second ? c - half : c;
+      Load4(cos_p + i, cs);
+      Load4(cos_p + i + 4, cs + 4);
+      Load4(sin_p + i, sn);
+      Load4(sin_p + i + 4, sn + 4);
+      if (!second) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sn[e] = -sn[e];
+      }
+    }
   }
-  const int partner = a.interleaved ? lane : (c < half ? lane + half / 8 : c < a.rot ? lane - half / 8 : lane);
+  const int partner = !in ? lane : second ? lane - half / 8 : lane + half / 8;
+  QT* const q_out = static_cast<QT*>(a.q_out) + static_cast<int64_t>(t) * a.H * a.D;
+  const int64_t kv_row = static_cast<int64_t>(slot) * a.Hkv * a.D;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int h = h0 + u * kGroups;
-    const bool there = h < slots;
-    const HeadSlot<XT, QT, KVT> s(a, t, there ? h : 0, slot);
+    const bool query = h < a.H, key = !query && h < a.H + a.Hkv;
     float v[8];
     Widen(raw[u], v);
-    const float* gain = there ? s.gain : nullptr;
     if (a.q_gain != nullptr) {  // the same for every lane of the grid: values, which are not normed, go along
       float sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
 #pragma unroll
       for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (gain != nullptr && mine) {
-        const float rsq = __frsqrt_rn(__fadd_rn(__fdiv_rn(sum, static_cast<float>(a.D)), a.eps));
-        const float4 g0 = __ldg(reinterpret_cast<const float4*>(gain + c)), g1 = __ldg(reinterpret_cast<const float4*>(gain + c) + 1);
-        const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+      if ((query || key) && mine) {
+        const float rsq = rsqrtf(fmaf(sum, inv_d, a.eps));
+        const float* const gain = (query ? a.q_gain : a.k_gain) + c;
+        float g[8];
+        Load4(gain, g);
+        Load4(gain + 4, g + 4);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = __fmul_rn(__fmul_rn(v[e], rsq), g[e]);
+        for (int e = 0; e < 8; ++e) v[e] = v[e] * rsq * g[e];
       }
     }
     float w[8];
+    if (a.interleaved) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = a.interleaved ? v[e ^ 1] : __shfl_sync(0xffffffffu, v[e], partner);
-    if (there && s.rotate) {
+      for (int e = 0; e < 8; ++e) w[e] = v[e ^ 1];
+    } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c + e < a.rot) v[e] = __fadd_rn(__fmul_rn(v[e], cs[e]), __fmul_rn(w[e], sn[e]));
+      for (int e = 0; e < 8; ++e) w[e] = __shfl_sync(0xffffffffu, v[e], partner);
     }
-    if (there && mine) {
-      if (s.q_dst != nullptr) Store8(s.q_dst + c, v);
-      else if (s.kv_dst != nullptr) Store8(s.kv_dst + c, v);
+    if ((query || key) && in) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e], cs[e], w[e] * sn[e]);
+    }
+    if (!mine) continue;
+    if (query) {
+      Store8(q_out + h * a.D + c, v);
+    } else if (written && h < a.H + 2 * a.Hkv) {
+      KVT* const pool = static_cast<KVT*>(key ? a.kc : a.vc) + kv_row;
+      Store8(pool + (key ? h - a.H : h - a.H - a.Hkv) * a.D + c, v);
     }
   }
 }
 
-// Whole words everywhere: heads of multiples of 8 channels up to 256, halves of the rotated part too (pairs beside one another need none), addresses and strides of 16 bytes.
+// Whole words everywhere: heads of multiples of 8 channels up to 256, the rotated part (its halves, where they make the pairs) too, addresses and strides of 16 bytes.
 bool FastApplies(const NormRopeArgs& a, size_t x_bytes)
 {
   auto words = [&](int64_t ld) { return ld * x_bytes % 16 == 0; };
-  return !a.faithful && a.D % 8 == 0 && a.D <= 256 && (a.interleaved || a.rot % 16 == 0) && Aligned16(a.q) && Aligned16(a.k) && Aligned16(a.v) && words(a.ld_q) &&
+  return !a.faithful && a.D % 8 == 0 && a.D <= 256 && a.rot % (a.interleaved ? 8 : 16) == 0 && static_cast<long long>(a.T) * (a.H + 2ll * a.Hkv) < (1ll << 31) && static_cast<long long>(a.H) * a.D < (1ll << 31) &&
+         Aligned16(a.cos_t) && Aligned16(a.sin_t) && Aligned16(a.q) && Aligned16(a.k) && Aligned16(a.v) && words(a.ld_q) &&
          words(a.ld_k) && words(a.ld_v) && Aligned16(a.q_out) && Aligned16(a.kc) && Aligned16(a.vc) && Aligned16(a.q_gain) && Aligned16(a.k_gain);
 }
 
@@ -237,10 +270,12 @@ cudaError_t LaunchFast(const NormRopeArgs& a, cudaStream_t st)
 {
   // Four groups of heads a warp while that leaves every SM sixteen warps; few tokens are bound by latency and take one.
   const int slots = a.H + 2 * a.Hkv, per_warp = 32 / L;
-  if (static_cast<long long>(a.T) * slots / (4 * per_warp) >= 148 * 16) {
-    return LaunchChained(NormRopeFast<XT, QT, KVT, L, 4>, dim3(a.T, (slots + 4 * per_warp * kFastWarps - 1) / (4 * per_warp * kFastWarps)), 32 * kFastWarps, 0, st, a);
-  }
-  return LaunchChained(NormRopeFast<XT, QT, KVT, L, 1>, dim3(a.T, (slots + per_warp * kFastWarps - 1) / (per_warp * kFastWarps)), 32 * kFastWarps, 0, st, a);
+  const bool many = static_cast<long long>(a.T) * slots / (4 * per_warp) >= 148 * 16;
+  const int chunks = (slots + (many ? 4 : 1) * per_warp - 1) / ((many ? 4 : 1) * per_warp);
+  const unsigned grid = static_cast<unsigned>((static_cast<long long>(a.T) * chunks + kFastWarps - 1) / kFastWarps);
+  const float inv_d = 1.f / static_cast<float>(a.D);
+  return many ? LaunchChained(NormRopeFast<XT, QT, KVT, L, 4>, grid, 32 * kFastWarps, 0, st, a, chunks, inv_d)
+              : LaunchChained(NormRopeFast<XT, QT, KVT, L, 1>, grid, 32 * kFastWarps, 0, st, a, chunks, inv_d);
 }
 
 template <typename XT, typename QT, typename KVT>

@@ -60,19 +60,21 @@ def _together(op: str, like: torch.Tensor, *ts) -> None:
     """Operands of one call: contiguous, on the device of `like`."""
     device = like.get_device()
     for t in ts:
-        if t is not None and (not t.is_cuda or t.get_device() != device or not t.is_contiguous()):
+        if t is not None and (t.get_device() != device or not t.is_cuda or not t.is_contiguous()):
             raise ValueError(f"{op}: operands must be contiguous CUDA tensors on {like.device} (there is no CPU path)")
 
 
 def _launch(like: torch.Tensor, function, *args) -> None:
     """function(*args, stream) on the current stream of the device of `like`, with that device current."""
-    stream = _stream(like)
     device = like.get_device()
-    if device == torch._C._cuda_getDevice():
-        N.check(function(*args, stream))
+    if device >= 0 and device == torch._C._cuda_getDevice():
+        status = function(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
+        stream = _stream(like)
         with torch.cuda.device(device):
-            N.check(function(*args, stream))
+            status = function(*args, stream)
+    if status != 0:
+        N.check(status)
 
 
 def init() -> None:
@@ -135,33 +137,39 @@ def shared_prefix_attention(query, key_cache, value_cache, prefix_tables, prefix
     prefix_tables[g] and then its own seq_lens[r] positions of block_tables (one table per row, or per equal group of consecutive rows).  Each prefix is read once
     for all of its rows.  See include/tlaloc_b200.h."""
     op = "SHARED_PREFIX_ATTENTION"
-    if query.dim() != 3 or key_cache.dim() != 4 or value_cache.shape != key_cache.shape or key_cache.shape[3] != query.shape[2]:
-        raise ValueError(f"{op}: query [R, H, D] and pools [P, bs, Hkv, D] are needed, got {tuple(query.shape)}, {tuple(key_cache.shape)}, {tuple(value_cache.shape)}")
-    if prefix_tables.dim() != 2 or block_tables.dim() != 2 or prefix_lens.dim() != 1 or row_starts.dim() != 1 or seq_lens.dim() != 1:
-        raise ValueError(f"{op}: prefix_tables [G, blocks], prefix_lens [G], row_starts [G + 1], block_tables [Tb, blocks] and seq_lens [R] are needed")
-    R, H, D = query.shape
-    P, bs, Hkv, _ = key_cache.shape
-    G, Mp = prefix_tables.shape
-    if prefix_lens.shape[0] != G or row_starts.shape[0] != G + 1 or seq_lens.shape[0] != R:
-        raise ValueError(f"{op}: {G} prefixes have as many lengths and one more row start, {R} rows as many lengths; got {prefix_lens.shape[0]}, {row_starts.shape[0]}, "
-                         f"{seq_lens.shape[0]}")
-    if value_cache.dtype != key_cache.dtype:
-        raise TypeError(f"{op}: the pools have one type, got {key_cache.dtype} and {value_cache.dtype}")
+    shape, pool_shape, prefix_shape, table_shape = query.shape, key_cache.shape, prefix_tables.shape, block_tables.shape
+    if len(shape) != 3 or len(pool_shape) != 4 or value_cache.shape != pool_shape or pool_shape[3] != shape[2]:
+        raise ValueError(f"{op}: query [R, H, D] and pools [P, bs, Hkv, D] are needed, got {tuple(shape)}, {tuple(pool_shape)}, {tuple(value_cache.shape)}")
+    if len(prefix_shape) != 2 or len(table_shape) != 2:
+        raise ValueError(f"{op}: prefix_tables [G, blocks] and block_tables [Tb, blocks] are needed")
+    R, H, D = shape
+    P, bs, Hkv, _ = pool_shape
+    G, Mp = prefix_shape
+    if prefix_lens.shape != (G,) or row_starts.shape != (G + 1,) or seq_lens.shape != (R,):
+        raise ValueError(f"{op}: {G} prefixes have as many lengths and one more row start, {R} rows as many lengths; got {tuple(prefix_lens.shape)}, "
+                         f"{tuple(row_starts.shape)}, {tuple(seq_lens.shape)}")
+    kind, pool_kind = query.dtype, key_cache.dtype
+    if value_cache.dtype != pool_kind:
+        raise TypeError(f"{op}: the pools have one type, got {pool_kind} and {value_cache.dtype}")
     for t in (prefix_tables, prefix_lens, row_starts, block_tables, seq_lens):
         if t.dtype != torch.int32:
             raise TypeError(f"{op}: tables, lengths and row starts are int32")
     _together(op, query, query, key_cache, value_cache, prefix_tables, prefix_lens, row_starts, block_tables, seq_lens)
     if out is None:
-        out = torch.empty((R, H, D), dtype=query.dtype if out_dtype is None else out_dtype, device=query.device)
-    _out(f"{op} out", out, (R, H, D), (torch.float32, torch.bfloat16), query)
+        out_dtype = kind if out_dtype is None else out_dtype
+        if out_dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"{op}: out_dtype is float32 or bfloat16, not {out_dtype}")
+        out = torch.empty(shape, dtype=out_dtype, device=query.device)
+    else:
+        _out(f"{op} out", out, shape, (torch.float32, torch.bfloat16), query)
     if scratch is None:
         scratch = shared_prefix_scratch(query, key_cache, prefix_tables, block_tables)
     else:
         _out(f"{op} scratch", scratch, None, torch.float32, query)
     lse = torch.empty((R, H), dtype=torch.float32, device=query.device) if return_lse else None
-    _launch(query, N.lib().tlaloc_b200_shared_prefix_attention, query.data_ptr(), _dt(query), key_cache.data_ptr(), value_cache.data_ptr(), _dt(key_cache),
-            prefix_tables.data_ptr(), prefix_lens.data_ptr(), row_starts.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), _dt(out), _ptr(lse),
-            scratch.data_ptr(), scratch.numel() * 4, R, H, D, P, bs, Hkv, G, Mp, block_tables.shape[1], block_tables.shape[0], float(scale))
+    _launch(query, N.lib().tlaloc_b200_shared_prefix_attention, query.data_ptr(), _DT.get(kind, -1), key_cache.data_ptr(), value_cache.data_ptr(), _DT.get(pool_kind, -1),
+            prefix_tables.data_ptr(), prefix_lens.data_ptr(), row_starts.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), _DT[out.dtype], _ptr(lse),
+            scratch.data_ptr(), scratch.numel() * 4, R, H, D, P, bs, Hkv, G, Mp, table_shape[1], table_shape[0], scale)
     return (out, lse) if return_lse else out
 
 
@@ -300,37 +308,44 @@ def norm_rope_kv_write(q, k, v, positions, cos, sin, slot_mapping, key_cache, va
     at slot_mapping; returns the queries.  q, k, v: f32 or bf16, rows of dense heads that may be column blocks of one projection; cos, sin f32 [positions, pairs]
     (rotary.pair_tables); pairs are (i, i + pairs), or (2i, 2i + 1) with `interleaved`.  See include/tlaloc_b200.h."""
     op = "NORM_ROPE_KV_WRITE"
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or key_cache.dim() != 4 or value_cache.shape != key_cache.shape:
+    shape, kv_shape, pool_shape = q.shape, k.shape, key_cache.shape
+    if len(shape) != 3 or len(kv_shape) != 3 or v.shape != kv_shape or len(pool_shape) != 4 or value_cache.shape != pool_shape:
         raise ValueError(f"{op}: q [T, H, hd], k and v [T, Hkv, hd] and pools [P, bs, Hkv, hd] are needed")
-    T, H, hd = q.shape
-    Hkv = k.shape[1]
-    P, bs = key_cache.shape[:2]
-    if k.shape[0] != T or k.shape[2] != hd or key_cache.shape[2] != Hkv or key_cache.shape[3] != hd:
-        raise ValueError(f"{op}: q {tuple(q.shape)}, k and v {tuple(k.shape)}, pools {tuple(key_cache.shape)} do not fit")
+    T, H, hd = shape
+    Tk, Hkv, hdk = kv_shape
+    P, bs, Hp, hdp = pool_shape
+    if Tk != T or hdk != hd or Hp != Hkv or hdp != hd:
+        raise ValueError(f"{op}: q {tuple(shape)}, k and v {tuple(kv_shape)}, pools {tuple(pool_shape)} do not fit")
+    device = q.get_device()
     lds = []
     for t, heads in ((q, H), (k, Hkv), (v, Hkv)):
         row, head, one = t.stride()
-        if not t.is_cuda or t.get_device() != q.get_device() or (one != 1 and hd > 1) or (head != hd and heads > 1):
+        if not t.is_cuda or t.get_device() != device or (one != 1 and hd > 1) or (head != hd and heads > 1):
             raise ValueError(f"{op}: q, k and v must be CUDA tensors on {q.device} with dense heads")
         lds.append(row if T > 1 else max(row, heads * hd))
-    if k.dtype != q.dtype or v.dtype != q.dtype or key_cache.dtype != value_cache.dtype:
+    kind, pool_kind = q.dtype, key_cache.dtype
+    if k.dtype != kind or v.dtype != kind or value_cache.dtype != pool_kind:
         raise TypeError(f"{op}: q, k and v have one type, and so have the pools")
-    if positions.dtype != torch.int32 or slot_mapping.dtype != torch.int32 or tuple(positions.shape) != (T,) or tuple(slot_mapping.shape) != (T,):
+    if positions.dtype != torch.int32 or slot_mapping.dtype != torch.int32 or positions.shape != (T,) or slot_mapping.shape != (T,):
         raise ValueError(f"{op}: positions and slot_mapping are int32 [{T}]")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape[0] < 1:
+    tables = cos.shape
+    if len(tables) != 2 or sin.shape != tables or cos.dtype != torch.float32 or sin.dtype != torch.float32 or tables[0] < 1:
         raise ValueError(f"{op}: cos and sin are f32 [positions, pairs]")
     for g in (q_gain, k_gain):
-        if g is not None and (g.dtype != torch.float32 or tuple(g.shape) != (hd,)):
+        if g is not None and (g.dtype != torch.float32 or g.shape != (hd,)):
             raise ValueError(f"{op}: gains are f32 [{hd}]")
     _together(op, q, positions, cos, sin, slot_mapping, key_cache, value_cache, q_gain, k_gain)
     if q_out is None:
         q_out = torch.empty((T, H, hd), dtype=q_dtype, device=q.device)
-    _out(f"{op} q_out", q_out, (T, H, hd), (torch.float32, torch.bfloat16), q)
+        if q_dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"{op}: q_dtype is float32 or bfloat16, not {q_dtype}")
+    else:
+        _out(f"{op} q_out", q_out, shape, (torch.float32, torch.bfloat16), q)
     if T == 0:
         return q_out
-    _launch(q, N.lib().tlaloc_b200_norm_rope_kv_write, q.data_ptr(), lds[0], k.data_ptr(), lds[1], v.data_ptr(), lds[2], _dt(q), _ptr(q_gain), _ptr(k_gain), float(eps),
-            positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), slot_mapping.data_ptr(), q_out.data_ptr(), _dt(q_out), key_cache.data_ptr(), value_cache.data_ptr(),
-            _dt(key_cache), T, H, Hkv, hd, 2 * cos.shape[1], int(interleaved), P * bs, cos.shape[0])
+    _launch(q, N.lib().tlaloc_b200_norm_rope_kv_write, q.data_ptr(), lds[0], k.data_ptr(), lds[1], v.data_ptr(), lds[2], _DT.get(kind, -1), _ptr(q_gain), _ptr(k_gain), eps,
+            positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), slot_mapping.data_ptr(), q_out.data_ptr(), _DT[q_out.dtype], key_cache.data_ptr(), value_cache.data_ptr(),
+            _DT.get(pool_kind, -1), T, H, Hkv, hd, 2 * tables[1], 1 if interleaved else 0, P * bs, tables[0])
     return q_out
 
 
@@ -361,29 +376,29 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     number for all rows or a tensor of one per row (f32; top_k i32).  A temperature that is not above 0 is greedy; top_k 0, top_p 1 and min_p 0 keep everything.  See
     include/tlaloc_b200.h."""
     op = "SAMPLE"
-    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.stride(1) != 1 and logits.shape[1] > 1):
-        raise ValueError(f"{op}: logits [rows, n] with dense rows are needed, got {tuple(logits.shape)}")
-    rows, n = logits.shape
-    if uniforms.dtype != torch.float32 or tuple(uniforms.shape) != (rows,):
+    shape, ld = logits.shape, logits.stride()
+    if len(shape) != 2 or shape[1] < 1 or (ld[1] != 1 and shape[1] > 1):
+        raise ValueError(f"{op}: logits [rows, n] with dense rows are needed, got {tuple(shape)}")
+    rows, n = shape
+    if uniforms.dtype != torch.float32 or uniforms.shape != (rows,):
         raise ValueError(f"{op}: uniforms are f32 [{rows}], got {uniforms.dtype} {tuple(uniforms.shape)}")
-    each, every = [], []
-    for name, setting, kind in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+    settings = [temperature, top_k, top_p, min_p]
+    each = [None, None, None, None]
+    for i, setting in enumerate(settings):
         if isinstance(setting, torch.Tensor):
-            if setting.dtype != kind or tuple(setting.shape) != (rows,):
-                raise ValueError(f"{op}: {name} of each row is {kind} [{rows}], got {setting.dtype} {tuple(setting.shape)}")
-            each.append(setting)
-            every.append(0)
-        else:
-            each.append(None)
-            every.append(max(-1, min(int(setting), 2**31 - 1)) if kind == torch.int32 else float(setting))
+            if setting.dtype != (torch.int32 if i == 1 else torch.float32) or setting.shape != (rows,):
+                raise ValueError(f"{op}: {('temperature', 'top_k', 'top_p', 'min_p')[i]} of each row is {torch.int32 if i == 1 else torch.float32} [{rows}], "
+                                 f"got {setting.dtype} {tuple(setting.shape)}")
+            each[i], settings[i] = setting, 0
     _together(op, logits, uniforms, *each)
     if out is None:
         out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
-    _out(f"{op} out", out, (rows,), torch.int32, logits)
+    else:
+        _out(f"{op} out", out, (rows,), torch.int32, logits)
     if rows == 0:
         return out
-    _launch(logits, N.lib().tlaloc_b200_sample, logits.data_ptr(), logits.stride(0) if rows > 1 else n, _dt(logits), uniforms.data_ptr(), *map(_ptr, each), *every,
-            out.data_ptr(), rows, n)
+    _launch(logits, N.lib().tlaloc_b200_sample, logits.data_ptr(), ld[0] if rows > 1 else n, _DT.get(logits.dtype, -1), uniforms.data_ptr(), *map(_ptr, each), float(settings[0]),
+            max(-1, min(int(settings[1]), 2**31 - 1)), float(settings[2]), float(settings[3]), out.data_ptr(), rows, n)
     return out
 
 
