@@ -176,16 +176,19 @@ struct MergeArgs {
 };
 
 constexpr int kMergeWarps = 4;
+constexpr int kMergeBatch = 8;  // records whose values are in flight together
 
-// A warp per (row, head); lane l owns channels l, l + 32, ...  The records in order: the prefix's by CTA, then the own slices; the same order in every run.
-template <typename OT>
+// A warp per (row, head); a lane owns the channel pairs lane, lane + 32, ...  The records in order: the prefix's by CTA, then the own slices; the same order in every
+// run.  Headers are read 32 at a time, a lane one, the first of them together with the first records' values: a merge takes about two trips to L2 beside the
+// plan's (one record after the other, each behind its header, 64 rows of 32 heads took 35 us where this takes 9).
+template <typename OT, int PAIRS>  // PAIRS channel pairs a lane: D <= 64 PAIRS
 __global__ void __launch_bounds__(32 * kMergeWarps) PrefixMerge(const __grid_constant__ MergeArgs a)
 {
   GridDependencySync();
   const int lane = threadIdx.x & 31;
   const long long rh = static_cast<long long>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5);
   if (rh >= static_cast<long long>(a.plan.R) * a.H) return;
-  const int row = static_cast<int>(rh / a.H), head = static_cast<int>(rh % a.H), kv = head / a.plan.group;
+  const int row = static_cast<int>(rh / a.H), head = static_cast<int>(rh - static_cast<long long>(row) * a.H), kv = head / a.plan.group;
   const int own = min((min(max(__ldg(a.lens + row), 0), a.max_own) + a.slice - 1) / a.slice, a.slices);
   PrefixLine line(a.plan);
   PrefixGroup g;
@@ -193,39 +196,91 @@ __global__ void __launch_bounds__(32 * kMergeWarps) PrefixMerge(const __grid_con
   size_t first = 0;
   const size_t own_step = static_cast<size_t>(a.plan.R) * a.H * (a.D + 2);
   if (line.Find(true, row, &g, &index) && g.tiles > 0) {
-    const int pair = (row - g.row0) * a.plan.group + head % a.plan.group;
-    const int unit = kv * g.units + pair / a.plan.unit_rows, work = g.work0 + unit * g.tiles;
+    const int pair = (row - g.row0) * a.plan.group + head - kv * a.plan.group, in_unit = pair / a.plan.unit_rows;
+    const int unit = kv * g.units + in_unit, work = g.work0 + unit * g.tiles;
     const int c0 = work / line.run, c1 = (work + g.tiles - 1) / line.run, block = c0 + g.unit0 + unit;
     if (block >= 0 && block + (c1 - c0) < a.plan.max_blocks) {
       shared = c1 - c0 + 1;
-      first = static_cast<size_t>(block) * a.plan.unit_rows + pair % a.plan.unit_rows;
+      first = static_cast<size_t>(block) * a.plan.unit_rows + pair - in_unit * a.plan.unit_rows;
     }
   }
-  const float* mine = a.own + static_cast<size_t>(rh) * (a.D + 2);
-  const int n = shared + own;
-  auto header = [&](int i) { return i < shared ? a.heads + 2 * (first + static_cast<size_t>(i) * a.plan.unit_rows) : mine + (i - shared) * own_step; };
-  auto values = [&](int i) { return i < shared ? a.acc + (first + static_cast<size_t>(i) * a.plan.unit_rows) * a.d8 : mine + (i - shared) * own_step + 2; };
-  float top = -INFINITY;
-  for (int i = lane; i < n; i += 32) top = fmaxf(top, header(i)[0]);
+  const float* const mine = a.own + static_cast<size_t>(rh) * (a.D + 2);
+  const int n = shared + own, pairs = a.D >> 1;
+  const size_t unit_rows = a.plan.unit_rows;
+  auto header = [&](int i) {
+    const float* h = i < shared ? a.heads + 2 * (first + i * unit_rows) : mine + (i - shared) * own_step;
+    return make_float2(h[0], h[1]);
+  };
+  auto values = [&](int i) { return i < shared ? a.acc + (first + i * unit_rows) * a.d8 : mine + (i - shared) * own_step + 2; };
+  const bool even = (a.D & 1) == 0;  // records start on 8-byte boundaries then
+  float2 v[kMergeBatch][PAIRS];
+  auto load_batch = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < kMergeBatch; ++u) {
+      const float* r = i0 + u < n ? values(i0 + u) : nullptr;
+#pragma unroll
+      for (int j = 0; j < PAIRS; ++j) {
+        const int p = lane + 32 * j;
+        v[u][j] = make_float2(0.f, 0.f);
+        if (r != nullptr && p < pairs) v[u][j] = even ? *reinterpret_cast<const float2*>(r + 2 * p) : make_float2(r[2 * p], r[2 * p + 1]);
+        else if (r != nullptr && p == pairs && !even) v[u][j].x = r[2 * p];  // the last channel of an odd head
+      }
+    }
+  };
+  float2 mine_h = lane < n ? header(lane) : make_float2(-INFINITY, 0.f);
+  load_batch(0);
+  float top = mine_h.x;
+  for (int i = lane + 32; i < n; i += 32) top = fmaxf(top, header(i).x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float sum = 0.f, acc[8] = {};
-  for (int i = 0; i < n; ++i) {
-    const float* h = header(i);
-    const float w = h[0] == -INFINITY ? 0.f : expf(h[0] - top);
-    if (w == 0.f) continue;
-    sum += w * h[1];
-    const float* v = values(i);
+  float sum = 0.f, acc[2 * PAIRS] = {};
+  for (int c0 = 0; c0 < n; c0 += 32) {
+    if (c0 > 0) mine_h = c0 + lane < n ? header(c0 + lane) : make_float2(-INFINITY, 0.f);
+    const float w_l = mine_h.x == -INFINITY ? 0.f : expf(mine_h.x - top), ws_l = w_l == 0.f ? 0.f : w_l * mine_h.y;
+    const int m = min(32, n - c0);
+    for (int i0 = 0; i0 < m; i0 += kMergeBatch) {
+      if (c0 + i0 > 0) load_batch(c0 + i0);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (lane + 32 * j < a.D) acc[j] += w * v[lane + 32 * j];
+      for (int u = 0; u < kMergeBatch; ++u) {
+        const float w = __shfl_sync(0xffffffffu, w_l, (i0 + u) & 31), ws = __shfl_sync(0xffffffffu, ws_l, (i0 + u) & 31);
+        if (i0 + u < m && w != 0.f) {  // uniform over the warp
+          sum += ws;
+#pragma unroll
+          for (int j = 0; j < PAIRS; ++j) {
+            acc[2 * j] += w * v[u][j].x;
+            acc[2 * j + 1] += w * v[u][j].y;
+          }
+        }
+      }
+    }
   }
-  OT* out = static_cast<OT*>(a.out) + rh * a.D;
+  OT* const out = static_cast<OT*>(a.out) + rh * a.D;
   const bool empty = sum == 0.f;  // no keys, or none that weighs anything
+  const bool whole = even && (reinterpret_cast<uintptr_t>(a.out) & 7) == 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (lane + 32 * j < a.D) out[lane + 32 * j] = FromF32<OT>(empty ? 0.f : acc[j] / sum);
+  for (int j = 0; j < PAIRS; ++j) {
+    const int p = lane + 32 * j;
+    const float x = empty ? 0.f : acc[2 * j] / sum, y = empty ? 0.f : acc[2 * j + 1] / sum;
+    if (p < pairs && whole) {
+      if constexpr (sizeof(OT) == 4) *reinterpret_cast<float2*>(out + 2 * p) = make_float2(x, y);
+      else *reinterpret_cast<__nv_bfloat162*>(out + 2 * p) = __floats2bfloat162_rn(x, y);
+    } else {
+      if (2 * p < a.D) out[2 * p] = FromF32<OT>(x);
+      if (2 * p + 1 < a.D) out[2 * p + 1] = FromF32<OT>(y);
+    }
+  }
   if (lane == 0 && a.lse != nullptr) a.lse[rh] = empty ? -INFINITY : top + logf(sum);
+}
+
+template <typename OT>
+cudaError_t LaunchMerge(const MergeArgs& m, cudaStream_t st)
+{
+  const unsigned blocks = static_cast<unsigned>((static_cast<long long>(m.plan.R) * m.H + kMergeWarps - 1) / kMergeWarps);
+  // An odd head's last channel is the first half of a pair of its own.
+  const int pairs = (m.D + 1) / 2;
+  return pairs <= 32   ? LaunchChained(PrefixMerge<OT, 1>, blocks, 32 * kMergeWarps, 0, st, m)
+         : pairs <= 64 ? LaunchChained(PrefixMerge<OT, 2>, blocks, 32 * kMergeWarps, 0, st, m)
+                       : LaunchChained(PrefixMerge<OT, 4>, blocks, 32 * kMergeWarps, 0, st, m);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -382,9 +437,7 @@ extern "C" int tlaloc_b200_shared_prefix_attention(const void* query, int32_t q_
   m.D = head_dim;
   m.d8 = a.d8;
   m.max_own = max_blocks_per_seq * block_size;
-  const unsigned blocks = static_cast<unsigned>((static_cast<long long>(num_rows) * num_heads + kMergeWarps - 1) / kMergeWarps);
-  e = out_dtype == TLALOC_B200_F32 ? LaunchChained(PrefixMerge<float>, blocks, 32 * kMergeWarps, 0, st, m)
-                                   : LaunchChained(PrefixMerge<__nv_bfloat16>, blocks, 32 * kMergeWarps, 0, st, m);
+  e = out_dtype == TLALOC_B200_F32 ? LaunchMerge<float>(m, st) : LaunchMerge<__nv_bfloat16>(m, st);
   if (e != cudaSuccess) return CudaFail("SHARED_PREFIX_ATTENTION merge launch", e);
   CountLaunches(2);
   return kOk;

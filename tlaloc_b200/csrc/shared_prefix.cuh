@@ -55,6 +55,11 @@ class PrefixLine {
   // The group that holds tile `at` of the line (by_row false), or query row `at` (by_row true); false if there is none.
   __device__ __forceinline__ bool Find(bool by_row, int at, PrefixGroup* found, int* index)
   {
+    if (p_.G == 1) {  // every lane has it
+      *found = mine_;
+      *index = 0;
+      return by_row ? at >= mine_.row0 && at < mine_.row0 + mine_.rows : at >= 0 && at < total;
+    }
     if (g0_ != 0) Load(0, 0, 0);
     for (;;) {
       const bool here = by_row ? at >= mine_.row0 && at < mine_.row0 + mine_.rows : at >= mine_.work0 && at < mine_.work0 + mine_.units * p_.Hkv * mine_.tiles;
@@ -104,7 +109,7 @@ class PrefixLine {
 
   __device__ __forceinline__ void Load(int g0, int unit_base, int work_base)
   {
-    const int lane = threadIdx.x & 31, g = g0 + lane;
+    const int lane = threadIdx.x & 31, g = p_.G == 1 ? 0 : g0 + lane;
     PrefixGroup r = {};
     if (g < p_.G) {
       const int a = min(max(__ldcg(p_.starts + g), 0), p_.R), b = min(max(__ldcg(p_.starts + g + 1), 0), p_.R);
@@ -115,6 +120,13 @@ class PrefixLine {
       r.tiles = (r.len + p_.tile - 1) / p_.tile;
     }
     const int units = r.units * p_.Hkv, work = units * r.tiles;
+    if (p_.G == 1) {
+      mine_ = r;
+      g0_ = 0;
+      unit_end_ = units;
+      work_end_ = work;
+      return;
+    }
     int u = units, w = work;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
