@@ -19,6 +19,25 @@ namespace {
 
 constexpr int kPairs = 64, kTileKeys = 32, kTiledThreads = 256;
 
+// Four channels from d on, zeros behind the head's end; `words`: heads are whole 16-byte words of f32 and their likes.
+__device__ __forceinline__ float4 Four(const float* p) { return __ldcg(reinterpret_cast<const float4*>(p)); }
+__device__ __forceinline__ float4 Four(const __nv_bfloat16* p)
+{
+  const uint2 w = __ldcg(reinterpret_cast<const uint2*>(p));
+  return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+}
+__device__ __forceinline__ float4 Four(const __nv_fp8_e4m3* p)
+{
+  const __nv_fp8x4_e4m3 w = *reinterpret_cast<const __nv_fp8x4_e4m3*>(p);
+  return static_cast<float4>(w);
+}
+template <typename T>
+__device__ __forceinline__ float4 Channels(const T* row, int d, int D, bool words)
+{
+  if (words) return d < D ? Four(row + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+  return make_float4(d < D ? ToF32(row[d]) : 0.f, d + 1 < D ? ToF32(row[d + 1]) : 0.f, d + 2 < D ? ToF32(row[d + 2]) : 0.f, d + 3 < D ? ToF32(row[d + 3]) : 0.f);
+}
+
 // Thread (ty, tx) of 16 x 16: scores of pairs 4 ty .. 4 ty + 3 with keys tx and tx + 16; outputs of the same pairs at channels tx + 16 j, j < NJ.
 template <typename QT, typename KVT, int NJ>
 __global__ void __launch_bounds__(kTiledThreads) PrefixTiled(const __grid_constant__ PrefixArgs a)
@@ -38,6 +57,8 @@ __global__ void __launch_bounds__(kTiledThreads) PrefixTiled(const __grid_consta
   const QT* q = static_cast<const QT*>(a.q);
   const KVT* kc = static_cast<const KVT*>(a.kc);
   const KVT* vc = static_cast<const KVT*>(a.vc);
+  const bool q_words = D % 4 == 0 && (reinterpret_cast<uintptr_t>(q) & (4 * sizeof(QT) - 1)) == 0;
+  const bool kv_words = D % 4 == 0 && ((reinterpret_cast<uintptr_t>(kc) | reinterpret_cast<uintptr_t>(vc)) & (4 * sizeof(KVT) - 1)) == 0;
   PrefixLine line(a.plan);
   int at = blockIdx.x * line.run;
   const int end = min(at + line.run, line.total);
@@ -56,9 +77,23 @@ __global__ void __launch_bounds__(kTiledThreads) PrefixTiled(const __grid_consta
     const PrefixSegment s = seg_s;
     auto row_of = [&](int pair) { return s.row0 + (s.pair0 + pair) / a.plan.group; };
     auto head_of = [&](int pair) { return s.kv * a.plan.group + (s.pair0 + pair) % a.plan.group; };
-    for (int i = tid; i < kPairs * ld; i += kTiledThreads) {
-      const int r = i / ld, d = i - r * ld;
-      qs[i] = r < s.pairs && d < D ? ToF32(q[(static_cast<size_t>(row_of(r)) * a.H + head_of(r)) * D + d]) * a.scale : 0.f;
+    // All of a thread's words in flight before the first is put down: one trip to memory instead of one for each.
+    constexpr int kQWords = kPairs * NJ * 4 / kTiledThreads, kKvWords = kTileKeys * NJ * 4 / kTiledThreads;  // of four channels, 16 NJ channels a row
+    constexpr int kAtOnce = kQWords < 8 ? kQWords : 8;
+#pragma unroll 1
+    for (int i0 = 0; i0 < kQWords; i0 += kAtOnce) {
+      float4 w[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int i = tid + (i0 + u) * kTiledThreads, r = i / (NJ * 4), d = i % (NJ * 4) * 4;
+        w[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < s.pairs && d < D) w[u] = Channels(q + (static_cast<size_t>(row_of(r)) * a.H + head_of(r)) * D, d, D, q_words);
+      }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int i = tid + (i0 + u) * kTiledThreads, r = i / (NJ * 4), d = i % (NJ * 4) * 4;
+        if (d < ld) *reinterpret_cast<float4*>(qs + r * ld + d) = make_float4(w[u].x * a.scale, w[u].y * a.scale, w[u].z * a.scale, w[u].w * a.scale);
+      }
     }
     if (tid < kPairs) {
       m_s[tid] = -INFINITY;
@@ -78,11 +113,28 @@ __global__ void __launch_bounds__(kTiledThreads) PrefixTiled(const __grid_consta
         off_s[tid] = ((static_cast<long long>(page) * a.bs + pos % a.bs) * a.plan.Hkv + s.kv) * D;
       }
       __syncthreads();
-      for (int i = tid; i < kTileKeys * ld; i += kTiledThreads) {  // positions past the end are zeros: 0 times whatever a page holds there must stay 0
-        const int r = i / ld, d = i - r * ld;
-        const bool live = r < n && d < D;
-        ks[i] = live ? ToF32(kc[off_s[r] + d]) : 0.f;
-        vs[i] = live ? ToF32(vc[off_s[r] + d]) : 0.f;
+      // Positions past the end are zeros: 0 times whatever a page holds there must stay 0.
+      constexpr int kFew = kKvWords < 4 ? kKvWords : 4;
+#pragma unroll 1
+      for (int i0 = 0; i0 < kKvWords; i0 += kFew) {
+        float4 kw[kFew], vw[kFew];
+#pragma unroll
+        for (int u = 0; u < kFew; ++u) {
+          const int i = tid + (i0 + u) * kTiledThreads, r = i / (NJ * 4), d = i % (NJ * 4) * 4;
+          kw[u] = vw[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (r < n && d < D) {
+            kw[u] = Channels(kc + off_s[r], d, D, kv_words);
+            vw[u] = Channels(vc + off_s[r], d, D, kv_words);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kFew; ++u) {
+          const int i = tid + (i0 + u) * kTiledThreads, r = i / (NJ * 4), d = i % (NJ * 4) * 4;
+          if (d < ld) {
+            *reinterpret_cast<float4*>(ks + r * ld + d) = kw[u];
+            *reinterpret_cast<float4*>(vs + r * ld + d) = vw[u];
+          }
+        }
       }
       __syncthreads();
       float sc[4][2] = {};

@@ -1,4 +1,5 @@
-// Records of shared prefixes on the tensor cores: bf16 pools, head sizes of multiples of 8 up to 128, pages of multiples of 8 positions.
+// Records of shared prefixes on the tensor cores: bf16 pools, head sizes of multiples of 8 up to 128, pages of multiples of 8 positions; e4m3fn pools, head sizes of
+// multiples of 16 up to 128, any pages.
 //
 // The (row, head) pairs that read one KV head of a prefix are the rows of a matrix product: S = Q K^T over tiles of 128 pairs x 128 keys, O += P V, both tcgen05.mma
 // kind::f16 with f32 accumulators in TMEM, keys and values by TMA out of their pages.  A CTA runs two streams, each with its own scores, weights (in the scores'
@@ -13,6 +14,8 @@
 // waits, read the queries twice as often and were no faster.
 // An f32 query enters as two bf16 parts.  Where the result is f32 the weights do as well (2^-17 of them is lost); for a bf16 result one part is enough: what is lost
 // (2^-9 of each weight, at random) is less than the result's own rounding.
+// e4m3fn rows: f16 holds every value, so both products are f16 x f16 (queries and weights as f16 parts), and the three warps that fill the ring read the rows with plain
+// loads, widen them and write them where TMA would have.
 // Every mbarrier wait is bounded.
 #include <cuda.h>
 
@@ -39,9 +42,9 @@ constexpr int kChain = 4;
 
 __device__ int g_prefix_status = 0;
 
-__host__ __device__ constexpr uint32_t InstrDesc(int n, bool b_mn_major)  // f32 accumulator, bf16, A K-major, M = 128
+__host__ __device__ constexpr uint32_t InstrDesc(int n, bool b_mn_major, bool f16)  // f32 accumulator, bf16 or f16 for both operands, A K-major, M = 128
 {
-  return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+  return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | (b_mn_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
 }
 __device__ __forceinline__ void TmaBox(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar)
 {
@@ -55,10 +58,28 @@ __device__ __forceinline__ float Exp2(float x)
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
 }
+// Two values as operands of the products, and what such a pair holds.
+template <bool F16>
 __device__ __forceinline__ uint32_t Pack(float a, float b)
 {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&v);
+  if constexpr (F16) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+template <bool F16>
+__device__ __forceinline__ float2 Unpack(uint32_t w)
+{
+  if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+// Four e4m3fn values as two pairs of f16.
+__device__ __forceinline__ void Widen(uint32_t w, uint32_t& a, uint32_t& b)
+{
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}\n" : "=r"(a), "=r"(b) : "r"(w));
 }
 // Two f32 at a time.
 __device__ __forceinline__ uint64_t Both(float a, float b)
@@ -86,8 +107,6 @@ __device__ __forceinline__ float Max3(float a, float b, float c)
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float Low(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float High(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 __device__ __forceinline__ void Store32(uint32_t dst, uint4 v)
 {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -110,7 +129,7 @@ __device__ __forceinline__ bool EitherWarp(int id, bool mine)
 }
 __device__ __forceinline__ void WarpsSync(int id) { asm volatile("bar.sync %0, 64;\n" ::"r"(id) : "memory"); }
 
-// ATOMS: 64-channel blocks of a head.  PLO: the weights in two parts.
+// ATOMS: 64-channel blocks of a head.  PLO: the weights in two parts.  F8: e4m3fn pools.
 template <typename QT, int ATOMS>
 struct PrefixTcLayout {
   static constexpr bool kQLo = sizeof(QT) == 4;
@@ -136,7 +155,7 @@ struct PrefixSteps {
   }
 };
 
-template <typename QT, int ATOMS, bool PLO>
+template <typename QT, int ATOMS, bool PLO, bool F8>
 __global__ void __launch_bounds__(kThreads, 1)
     PrefixTc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PrefixArgs a, const int box)
 {
@@ -185,7 +204,50 @@ __global__ void __launch_bounds__(kThreads, 1)
   PrefixSegment s;
   int items = 0;  // of the ring, in front of this segment: keys and values of its tiles in turn
 
-  if (warp > kWarps) {
+  if (F8 && warp > kWarps) {
+    constexpr int kWords = ATOMS * 4, kRowsAtOnce = 32 / kWords, kBatch = 8;  // 16-byte words of a row, rows of a warp's load, loads in flight
+    const int word = lane % kWords, sub = lane / kWords, shift = (a.bs & (a.bs - 1)) == 0 ? __ffs(a.bs) - 1 : -1;
+    int it = warp - kWarps - 1;
+    while (line.Next(end, &at, &s)) {
+      const int last = items + 2 * (s.tile1 - s.tile0);
+      const int* table = a.tables + static_cast<size_t>(s.index) * a.M;
+      for (; it < last; it += kProducers) {
+        const int sl = it % kSlots, use = it / kSlots, pos0 = (s.tile0 + ((it - items) >> 1)) * kKeys;
+        const uint8_t* const pool = static_cast<const uint8_t*>((it & 1) != 0 ? a.vc : a.kc) + s.kv * a.D + word * 16;
+        if (use > 0) ok = MbarWaitWarp(empty + 8 * sl, (use - 1) & 1, lane, abort_word) && ok;
+#pragma unroll 1
+        for (int r0 = sub; r0 < kKeys; r0 += kBatch * kRowsAtOnce) {
+          uint4 raw[kBatch];
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {  // zeros behind the prefix's end and the head's
+            const int pos = pos0 + r0 + u * kRowsAtOnce;
+            raw[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (pos < s.len && word * 16 < a.D) {
+              const int block = shift >= 0 ? pos >> shift : pos / a.bs;
+              const int page = min(max(__ldg(table + block), 0), a.P - 1);
+              raw[u] = __ldcg(reinterpret_cast<const uint4*>(pool + (static_cast<int64_t>(page) * a.bs + pos - block * a.bs) * (a.plan.Hkv * a.D)));
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            const int row = r0 + u * kRowsAtOnce;
+            uint4 lo, hi;
+            Widen(raw[u].x, lo.x, lo.y);
+            Widen(raw[u].y, lo.z, lo.w);
+            Widen(raw[u].z, hi.x, hi.y);
+            Widen(raw[u].w, hi.z, hi.w);
+            const uint32_t dst = ring + sl * kPart + (word >> 2) * kAtom + row * 128;
+            Store32(dst + ((((word & 3) * 2) ^ (row & 7)) << 4), lo);
+            Store32(dst + ((((word & 3) * 2 + 1) ^ (row & 7)) << 4), hi);
+          }
+        }
+        FenceAsync();
+        __syncwarp();
+        if (lane == 0) MbarArrive(full + 8 * sl);
+      }
+      items = last;
+    }
+  } else if (warp > kWarps) {
     const int boxes = kKeys / box, atom = lane / boxes, mine = lane - atom * boxes;  // up to 32 boxes an item: 16 of 8 positions by two atoms
     int it = warp - kWarps - 1;                                                       // this warp's next item
     while (line.Next(end, &at, &s)) {
@@ -216,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kWarps) {
     // One lane issues everything, between softmax warps that want the same issue slots: what it does besides waiting and issuing is kept to a minimum.
-    const uint32_t o_idesc = InstrDesc((a.D + 15) / 16 * 16, true);
+    const uint32_t o_idesc = InstrDesc((a.D + 15) / 16 * 16, true, F8);
     const uint64_t qd = SmemDesc(base, 16, 1024), kd = SmemDesc(ring, 16, 1024), vd = SmemDesc(ring, kAtom, 1024);
     const int depth = (a.D + 15) / 16;  // channels by 16
     uint32_t segment = 0;
@@ -237,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           return sl;
         };
-        const uint32_t s_idesc = InstrDesc(pair_tiles ? kKeys : kHalf, false);
+        const uint32_t s_idesc = InstrDesc(pair_tiles ? kKeys : kHalf, false, F8);
         auto scores = [&](int w, uint32_t sl) {
           // The weights of the step before lay here; their product is in front of these MMAs in the same queue.
           const uint32_t acc = tmem + w * 128;
@@ -307,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr int kChunks = ATOMS * 8, kPass = kWarps * 32 / kChunks;  // 16-byte words of a row; rows that the threads read at a time
       {
         const int c = tid % kChunks, first = tid / kChunks, n = steps.pair_tiles ? 2 * kRows : kRows;
-        constexpr int kAhead = 4;
+        constexpr int kAhead = Layout::kQLo ? 2 : 4;
         for (int p0 = first; p0 < n; p0 += kAhead * kPass) {
           uint4 raw[kAhead][Layout::kQLo ? 2 : 1];
 #pragma unroll
@@ -331,12 +393,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 x = __uint_as_float((e & 1) != 0 ? v.z : v.x), y = __uint_as_float((e & 1) != 0 ? v.w : v.y);
               } else {
                 const uint32_t v = e == 0 ? raw[u][0].x : e == 1 ? raw[u][0].y : e == 2 ? raw[u][0].z : raw[u][0].w;
-                x = Low(v), y = High(v);
+                const float2 two = Unpack<false>(v);
+                x = two.x, y = two.y;
               }
               x *= sign;
               y *= sign;
-              hi[e] = Pack(x, y);
-              lo[e] = Pack(x - Low(hi[e]), y - High(hi[e]));
+              hi[e] = Pack<F8>(x, y);
+              const float2 kept = Unpack<F8>(hi[e]);
+              lo[e] = Pack<F8>(x - kept.x, y - kept.y);
             }
             const uint32_t dst = base + (pair >> 7) * Layout::kQTile + (c >> 3) * kAtom + (pair & 127) * 128 + (((c & 7) ^ (pair & 7)) << 4);
             Store32(dst, make_uint4(hi[0], hi[1], hi[2], hi[3]));
@@ -448,8 +512,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               p0 = Exp2(p0);
               p1 = Exp2(p1);
               s2[(e >> 1) & 1] = Add2(s2[(e >> 1) & 1], Both(p0, p1));
-              hi[e / 2] = Pack(p0, p1);
-              if constexpr (PLO) lo[e / 2] = Pack(p0 - Low(hi[e / 2]), p1 - High(hi[e / 2]));
+              hi[e / 2] = Pack<F8>(p0, p1);
+              if constexpr (PLO) {
+                const float2 kept = Unpack<F8>(hi[e / 2]);
+                lo[e / 2] = Pack<F8>(p0 - kept.x, p1 - kept.y);
+              }
             }
             TcSt16(sa + 32 * c, hi);
             if constexpr (PLO) TcSt16(sa + 32 * c + 16, lo);
@@ -565,7 +632,8 @@ bool Encode(CUtensorMap* map, const void* pool, const PrefixArgs& a, int box)
 template <typename QT, int ATOMS, bool PLO>
 cudaError_t Prepare()
 {
-  return cudaFuncSetAttribute(PrefixTc<QT, ATOMS, PLO>, cudaFuncAttributeMaxDynamicSharedMemorySize, PrefixTcLayout<QT, ATOMS>::kBytes);
+  const cudaError_t e = cudaFuncSetAttribute(PrefixTc<QT, ATOMS, PLO, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PrefixTcLayout<QT, ATOMS>::kBytes);
+  return e == cudaSuccess ? cudaFuncSetAttribute(PrefixTc<QT, ATOMS, PLO, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PrefixTcLayout<QT, ATOMS>::kBytes) : e;
 }
 template <typename QT>
 cudaError_t PrepareBoth()
@@ -601,32 +669,35 @@ KernelSetup g_setup(PreparePrefixTc, ReadPrefixStatus);
 int BoxOf(int block_size) { return std::min(block_size & -block_size, kKeys); }
 
 template <typename QT, int ATOMS>
-cudaError_t Launch(const PrefixArgs& a, bool plo, cudaStream_t st)
+cudaError_t Launch(const PrefixArgs& a, bool plo, bool f8, cudaStream_t st)
 {
-  CUtensorMap map_k, map_v;
-  const int box = BoxOf(a.bs);
+  CUtensorMap map_k = {}, map_v = {};
+  const int box = BoxOf(a.bs), smem = PrefixTcLayout<QT, ATOMS>::kBytes;
+  if (f8) {
+    return plo ? LaunchChained(PrefixTc<QT, ATOMS, true, true>, a.plan.grid, kThreads, smem, st, map_k, map_v, a, box)
+               : LaunchChained(PrefixTc<QT, ATOMS, false, true>, a.plan.grid, kThreads, smem, st, map_k, map_v, a, box);
+  }
   if (!Encode(&map_k, a.kc, a, box) || !Encode(&map_v, a.vc, a, box)) return cudaErrorInvalidValue;
-  const int smem = PrefixTcLayout<QT, ATOMS>::kBytes;
-  return plo ? LaunchChained(PrefixTc<QT, ATOMS, true>, a.plan.grid, kThreads, smem, st, map_k, map_v, a, box)
-             : LaunchChained(PrefixTc<QT, ATOMS, false>, a.plan.grid, kThreads, smem, st, map_k, map_v, a, box);
+  return plo ? LaunchChained(PrefixTc<QT, ATOMS, true, false>, a.plan.grid, kThreads, smem, st, map_k, map_v, a, box)
+             : LaunchChained(PrefixTc<QT, ATOMS, false, false>, a.plan.grid, kThreads, smem, st, map_k, map_v, a, box);
 }
 
 }  // namespace
 
 bool PrefixTcApplies(const PrefixArgs& a, int q_dtype, int kv_dtype)
 {
-  return kv_dtype == TLALOC_B200_BF16 && IsFloatType(q_dtype) && a.D >= 8 && a.D <= 128 && a.D % 8 == 0 && a.bs % 8 == 0 && Aligned16(a.q) && Aligned16(a.kc) &&
-         Aligned16(a.vc) && static_cast<long long>(a.P) * a.bs < (1ll << 31) && TensorMapEncoder() != nullptr;
+  if (!IsFloatType(q_dtype) || a.D < 8 || a.D > 128 || a.D % 8 != 0 || !Aligned16(a.q) || !Aligned16(a.kc) || !Aligned16(a.vc)) return false;
+  if (kv_dtype == TLALOC_B200_F8E4M3FN) return a.D % 16 == 0 && static_cast<long long>(a.plan.Hkv) * a.D < (1ll << 31);
+  return kv_dtype == TLALOC_B200_BF16 && a.bs % 8 == 0 && static_cast<long long>(a.P) * a.bs < (1ll << 31) && TensorMapEncoder() != nullptr;
 }
 
 cudaError_t LaunchPrefixTc(const PrefixArgs& a, int q_dtype, int kv_dtype, int out_dtype, cudaStream_t st)
 {
-  (void)kv_dtype;
   const cudaError_t e = PreparePrefixTc();
   if (e != cudaSuccess) return e;
-  const bool plo = out_dtype == TLALOC_B200_F32;
-  if (q_dtype == TLALOC_B200_F32) return a.D <= 64 ? Launch<float, 1>(a, plo, st) : Launch<float, 2>(a, plo, st);
-  return a.D <= 64 ? Launch<__nv_bfloat16, 1>(a, plo, st) : Launch<__nv_bfloat16, 2>(a, plo, st);
+  const bool plo = out_dtype == TLALOC_B200_F32, f8 = kv_dtype == TLALOC_B200_F8E4M3FN;
+  if (q_dtype == TLALOC_B200_F32) return a.D <= 64 ? Launch<float, 1>(a, plo, f8, st) : Launch<float, 2>(a, plo, f8, st);
+  return a.D <= 64 ? Launch<__nv_bfloat16, 1>(a, plo, f8, st) : Launch<__nv_bfloat16, 2>(a, plo, f8, st);
 }
 
 }  // namespace tlaloc_b200
