@@ -10,11 +10,11 @@
 //
 // A cluster of CTAs shares a row; each reads its part once and keeps it in shared memory where it fits.  Passes over the part:
 //   1  the largest value
-//   2  (with top-k or top-p) how many values, and roughly which mass, lie in each of 1024 bins of (max - x) / T, and for top-p the exact mass of all
+//   2  (with top-k or top-p) how many values lie in each of 1024 bins of (max - x) / T, a sixteenth of an octave of w each, and for top-p the exact mass of all
 //   3  where the bins from the largest value down to the edge hold no more than 512 values, as they mostly do: these go to one CTA, which ranks them, a thread each, and
 //      finds both edges and the token among them
-//   Otherwise, per edge: the exact count and mass above the bin that it lies in; the bin's values go to one CTA, which ranks them and finds the edge.  The rough masses
-//      of pass 2 only say where to look: the exact ones decide, and move on to a neighbouring bin if they must.  A bin with more values than a CTA ranks is halved by
+//   Otherwise, per edge: the exact count and mass above the bin that it lies in; the bin's values go to one CTA, which ranks them and finds the edge.  Rough masses
+//      (a bin's count times its middle w) only say where to look: the exact ones decide, and move on to a neighbouring bin if they must.  A bin with more values than a CTA ranks is halved by
 //      value, over and over (equal logits by the thousand).  Then
 //   4  the mass that is kept, by warp, and the draw, in the one warp whose stretch it falls into
 // Without top-k and top-p there are passes 1 and 4 alone, which the f64 units bound: nine operations an exponential.
@@ -58,32 +58,34 @@ __device__ __forceinline__ uint32_t KeyOf(float x)
 }
 __device__ __forceinline__ float ValueOf(uint32_t key) { return __uint_as_float(key ^ ((key >> 31) != 0u ? 0x80000000u : 0xffffffffu)); }
 
-// exp(d) for d <= 0 by a table of 2^(j / 256) and a polynomial of degree 4 in what is left, |r| <= ln 2 / 512 (Tang, "Table-driven implementation of the exponential function",
-// 1989): the first term left out is r^5 / 120 = 4e-17 of the result.  Nine f64 operations instead of the library's twenty; below 2^-1000 the result is 0.
+// 2^t for -1000 <= t <= 0 by a table of 2^(j / 256) and a polynomial of degree 4 in what is left, |r| <= 1 / 512 (Tang, "Table-driven implementation of the exponential
+// function", 1989): the first term left out is (r ln 2)^5 / 120 = 4e-17 of the result.  Eight f64 operations instead of the library's twenty.
 constexpr int kExpTable = 256;
-__device__ __forceinline__ double TableExp2(double t, const double* table)  // 2^t, t <= 0
+__device__ __forceinline__ double TableExp2(double t, const double* table)
 {
-  if (t < -1000.0) return 0.0;
   constexpr double kRound = 6755399441055744.0 / kExpTable;  // 1.5 * 2^52 / 256: its last place is 1 / 256
+  constexpr double kLn2 = 0.69314718055994530942;
   const double shifted = t + kRound;
   const int k = __double2loint(shifted);  // t * 256 rounded, in the low word
-  const double r = (t - (shifted - kRound)) * 0.69314718055994530942;
-  const double p = fma(fma(fma(fma(r, 1.0 / 24, 1.0 / 6), r, 0.5), r, 1.0), r, 1.0);
+  const double r = t - (shifted - kRound);
+  const double p = fma(fma(fma(fma(r, kLn2 * kLn2 * kLn2 * kLn2 / 24, kLn2 * kLn2 * kLn2 / 6), r, kLn2 * kLn2 / 2), r, kLn2), r, 1.0);
   const double scaled = table[k & (kExpTable - 1)] * p;
   return __hiloint2double(__double2hiint(scaled) + ((k >> 8) << 20), __double2loint(scaled));
 }
 
 template <typename XT>
-__global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_constant__ SampleArgs a)
+__global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_constant__ SampleArgs a)
 {
   extern __shared__ __align__(16) unsigned char part_raw[];  // this CTA's part of the row, where it fits
   __shared__ double table[kExpTable];
   __shared__ double red[kSampleWarps], told_mass[kMaxRanks], warp_mass[kSampleWarps];
+  __shared__ float fred[kSampleWarps];
   __shared__ double told_masses[2][kMaxRanks];
   __shared__ int ired[kSampleWarps], told_count[kMaxRanks], told_counts[2][kMaxRanks];
   __shared__ uint32_t kred[kSampleWarps], told_key[kMaxRanks], range_s[2];
   __shared__ int bin_count[kBins];
-  __shared__ __align__(16) float bin_mass[kBins];
+  __shared__ double s_weight[kRanked];
+  __shared__ int s_order[kRanked];
   __shared__ uint32_t cand_key[kRanked];
   __shared__ int cand_index[kRanked];
   __shared__ int cand_n, cand_token, cand_last, cand_done;
@@ -130,7 +132,7 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
 
   // 1: the largest value, and the part into shared memory.
   XT* const part = reinterpret_cast<XT*>(part_raw);
-  uint32_t best = 0;
+  float most = -INFINITY;  // fmaxf passes NaN by
   {
     constexpr int kPer = 16 / static_cast<int>(sizeof(XT));
     const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
@@ -147,18 +149,17 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
         if (a.on_chip) reinterpret_cast<uint4*>(part)[i0 + e * kSampleThreads] = raw[e];
         const XT* v = reinterpret_cast<const XT*>(&raw[e]);
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) best = max(best, KeyOf(ToF32(v[k])));
+        for (int k = 0; k < kPer; ++k) most = fmaxf(most, ToF32(v[k]));
       }
     }
     for (int i = words * kPer + tid; i < n; i += kSampleThreads) {
       const XT v = x[i];
       if (a.on_chip) part[i] = v;
-      best = max(best, KeyOf(ToF32(v)));
+      most = fmaxf(most, ToF32(v));
     }
   }
   const XT* const v = a.on_chip ? part : x;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+  uint32_t best = __reduce_max_sync(0xffffffffu, KeyOf(most));
   if (lane == 0) kred[warp] = best;
   __syncthreads();  // the part is there, too
   for (int w = 0; w < kSampleWarps; ++w) best = max(best, kred[w]);
@@ -193,10 +194,12 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
 
   const double scale = 1.4426950408889634074 / static_cast<double>(temperature), dtop = static_cast<double>(top);
   const bool infinite = top == INFINITY;
+  // Values from here down (and NaN) weigh nothing: 2^-1000, or anything beside infinity.
+  const double low = dtop - 1000.0 / scale;
+  const float cut = infinite ? top : low < -3.4028234663852886e38 ? -INFINITY : static_cast<float>(low);
   auto weight = [&](float f) -> double {  // 1 for the largest: 2^0 is exact
-    if (infinite) return f == INFINITY ? 1.0 : 0.0;
-    if (!(f == f)) return 0.0;
-    return TableExp2((static_cast<double>(f) - dtop) * scale, table);
+    const double w = TableExp2((static_cast<double>(f) - dtop) * scale, table);
+    return f > cut ? w : f == top ? 1.0 : 0.0;
   };
   // A lane's values [i, i + kVec) of the part, -infinity behind its end.
   constexpr int kVec = 16 / static_cast<int>(sizeof(XT));
@@ -228,53 +231,38 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
     return static_cast<int>(fminf((top - f) * fscale, static_cast<float>(kBins - 1)));
   };
 
+  const double least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
+  // What a thread's stretch keeps of the bins above `above_bin`, once that has been added up on the way to an edge in it.
+  int above_bin = -1;
+  double above_mine = 0.0;
   // Kept: keys above edge_key, and of those equal to it the ones up to edge_index.
   uint32_t edge_key = 0;
   int edge_index = a.n;
   const bool by_k = top_k > 0 && top_k < a.n, by_p = top_p < 1.f;
   if (by_k || by_p) {
     // 2: the bins, and the mass of all.
-    for (int i = tid; i < kBins; i += kSampleThreads) {
-      bin_count[i] = 0;
-      bin_mass[i] = 0.f;
-    }
+    for (int i = tid; i < kBins; i += kSampleThreads) bin_count[i] = 0;
     __syncthreads();
     double all = 0.0;
     each([&](int, float f) {
-      const int b = bin_of(f);
-      atomicAdd(&bin_count[b], 1);
-      if (by_p) {
-        const double w = weight(f);
-        all += w;
-        atomicAdd(&bin_mass[b], static_cast<float>(w));
-      }
+      atomicAdd(&bin_count[bin_of(f)], 1);
+      if (by_p) all += weight(f);
     });
     if (by_p) all = cluster_sum(all, red, told_mass);
-    auto add_bins = [&]() {  // the row's bins: every rank adds up an equal share of them over all ranks and tells everyone
-      __syncthreads();
-      if (ranks == 1) return;
+    if (ranks > 1) {  // the row's bins: every rank adds up an equal share of them over all ranks and tells everyone
       cluster.sync();
       const int share = kBins / ranks, b = rank * share + tid;
       int c = 0;
-      float m = 0.f;
-      if (tid < share) {
-        for (int q = 0; q < ranks; ++q) {
-          c += *cluster.map_shared_rank(bin_count + b, q);
-          m += *cluster.map_shared_rank(bin_mass + b, q);
-        }
-      }
+      if (tid < share)
+        for (int q = 0; q < ranks; ++q) c += *cluster.map_shared_rank(bin_count + b, q);
       cluster.sync();
-      if (tid < share) {
-        for (int q = 0; q < ranks; ++q) {
-          *cluster.map_shared_rank(bin_count + b, q) = c;
-          *cluster.map_shared_rank(bin_mass + b, q) = m;
-        }
-      }
+      if (tid < share)
+        for (int q = 0; q < ranks; ++q) *cluster.map_shared_rank(bin_count + b, q) = c;
       cluster.sync();
-    };
-    add_bins();
-    bool redo = false;
-    // The first bin at whose end `enough(count, mass)` holds, the last one if it never does; *upto: the count there.
+    } else {
+      __syncthreads();
+    }
+    // The first bin at whose end `enough(count, rough mass, rough mass of all)` holds, the last one if it never does; *upto: the count there.
     auto find_bin = [&](auto&& enough, int* upto) {
       __shared__ int found_s, upto_s;
       __shared__ int cs[kSampleWarps];
@@ -287,7 +275,7 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
         ct += bin_count[tid * kEach + e];
-        mt += bin_mass[tid * kEach + e];
+        mt += static_cast<float>(bin_count[tid * kEach + e]) * exp2f(-(static_cast<float>(tid * kEach + e) + 0.5f) / kBinsPerOctave);  // as if all were in its middle: within 2.2 %
         c[e] = ct;
         m[e] = mt;
       }
@@ -311,13 +299,17 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
       __syncthreads();
       int cb = cu - ct;
       float mb = mu - mt;
-      for (int w = 0; w < warp; ++w) {
-        cb += cs[w];
-        mb += ms[w];
+      float total = 0.f;
+      for (int w = 0; w < kSampleWarps; ++w) {
+        if (w < warp) {
+          cb += cs[w];
+          mb += ms[w];
+        }
+        total += ms[w];
       }
 #pragma unroll
       for (int e = kEach - 1; e >= 0; --e)
-        if (enough(cb + c[e], mb + m[e])) atomicMin(&found_s, tid * kEach + e);
+        if (enough(cb + c[e], mb + m[e], total)) atomicMin(&found_s, tid * kEach + e);
       __syncthreads();
       const int b = found_s;
       if (tid == b / kEach) upto_s = cb + (b % kEach == 0 ? c[0] : c[kEach - 1]);
@@ -329,11 +321,11 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
     static_assert(kBins / kSampleThreads == 2, "find_bin: two bins a thread");
 
     // Everything down to the edge in rank 0, if that is few enough.
-    const double least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
     {
       int few = 0;
-      const float rough = static_cast<float>(static_cast<double>(top_p) * all) * 1.001f;
-      const int b = by_k ? find_bin([&](int c, float) { return c >= top_k; }, &few) : find_bin([&](int, float m) { return m >= rough; }, &few);
+      // For top-p a tenth of what may be left out is taken as well, so that rough masses rarely stop short.
+      const float upto = top_p > 0.f ? top_p + 0.1f * (1.f - top_p) : 0.1f;
+      const int b = by_k ? find_bin([&](int c, float, float) { return c >= top_k; }, &few) : find_bin([&](int, float m, float total) { return m >= upto * total; }, &few);
       if (few <= kRanked) {
         if (tid == 0) cand_n = 0;
         cluster.sync();
@@ -348,10 +340,8 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
         });
         cluster.sync();
         if (rank == 0) {
-          // By rank, in the bins' place: index, then weight.
-          int* const s_index = bin_count;
-          double* const s_weight = reinterpret_cast<double*>(bin_mass);
-          static_assert(sizeof(bin_mass) >= sizeof(double) * kRanked && kRanked == kSampleThreads, "a thread a value");
+          int* const s_index = s_order;  // by rank: index, weight
+          static_assert(kRanked == kSampleThreads, "a thread a value");
           const int m = cand_n;
           if (tid < m) {
             const uint32_t key = cand_key[tid];
@@ -403,25 +393,8 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
         }
         cluster.sync();
         if (cand_done != 0) return;
-        // The bins are gone where they were ranked: take them from a rank that has them (there is one, or they are counted again).
-        redo = true;
       }
     }
-    if (redo) {
-      cluster.sync();
-      for (int i = tid; i < kBins; i += kSampleThreads) {
-        bin_count[i] = 0;
-        bin_mass[i] = 0.f;
-      }
-      __syncthreads();
-      each([&](int, float f) {
-        const int b = bin_of(f);
-        atomicAdd(&bin_count[b], 1);
-        atomicAdd(&bin_mass[b], static_cast<float>(weight(f)));
-      });
-      add_bins();
-    }
-
     auto mass_upto_edge = [&]() {
       double m = 0.0;
       each([&](int i, float f) {
@@ -454,6 +427,12 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
       }
       cluster.sync();
     };
+    // What the rough masses say lies above a bin.
+    auto rough_above = [&](int b) {
+      float m = 0.f;
+      for (int i = tid; i < b; i += kSampleThreads) m += static_cast<float>(bin_count[i]) * exp2f(-(static_cast<float>(i) + 0.5f) / kBinsPerOctave);
+      return block_sum(m, fred);
+    };
     // The range over all ranks; cluster_sums, which follows it, parts this one's words from the next one's.
     auto cluster_range = [&](uint32_t& least_key, uint32_t& most_key) {
       least_key = __reduce_min_sync(0xffffffffu, least_key);
@@ -472,42 +451,54 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
     // The edge in or next to bin `b`.  Counting: the value of rank `want_count`.  Otherwise: the last value whose betters hold less than `want_mass`, none beyond
     // (limit_key, limit_index).  kept_mass, if given: the exact mass of what is kept.
     auto find_edge = [&](int b, bool counting, int want_count, double want_mass, uint32_t limit_key, int limit_index, double* kept_mass) {
-      int moved = 0;  // which way: never back, whatever sums of the same values in two groupings say
+      int b_lo = 0, b_hi = limit_key != 0u ? bin_of(ValueOf(limit_key)) : kBins - 1;  // bins that the edge may lie in
       for (;;) {
         // Exactly what lies above the bin, and in it.
         int above_n = 0, in_n = 0;
         double above = 0.0, in = 0.0;
         uint32_t k_lo = 0xffffffffu, k_hi = 0;  // the bin's values lie between these keys
-        each([&](int i, float f) {
-          const int at = bin_of(f);
-          if (at > b) return;
-          const uint32_t key = KeyOf(f);
-          if (key < limit_key || (key == limit_key && lo + i > limit_index)) return;
-          const double w = counting ? 0.0 : weight(f);
-          if (at < b) {
-            ++above_n;
-            above += w;
-          } else {
-            ++in_n;
-            in += w;
-            k_lo = min(k_lo, key);
-            k_hi = max(k_hi, key);
+        above_mine = 0.0;
+        for (int i0 = w_lo + lane * kVec; i0 < w_hi; i0 += 32 * kVec) {
+          float f[kVec];
+          values(i0, w_hi, f);
+#pragma unroll
+          for (int k = 0; k < kVec; ++k) {
+            const int i = i0 + k, at = bin_of(f[k]);
+            if (i >= w_hi || at > b) continue;
+            const uint32_t key = KeyOf(f[k]);
+            if (at < b) {
+              const double w = counting ? 0.0 : weight(f[k]);
+              ++above_n;
+              above += w;
+              if (w >= least) above_mine += w;
+            } else if (key > limit_key || (key == limit_key && lo + i <= limit_index)) {
+              ++in_n;
+              if (!counting) in += weight(f[k]);
+              k_lo = min(k_lo, key);
+              k_hi = max(k_hi, key);
+            }
           }
-        });
+        }
+        above_bin = counting ? -1 : b;
         cluster_range(k_lo, k_hi);
         cluster_sums(above_n, in_n, above, in);
-        if (!counting && above_n > 0 && above >= want_mass) {  // roundings of the rough masses: the edge lies higher
-          if (moved <= 0) {
-            moved = -1;
-            --b;
+        if (!counting) {
+          // The edge lies higher or lower: the exact mass above this bin says by how much the rough ones are off.
+          const bool higher = above_n > 0 && above >= want_mass, lower = !higher && above + in < want_mass;
+          if (higher) b_hi = b - 1;
+          if (lower) b_lo = b + 1;
+          if ((higher || lower) && b_lo <= b_hi) {
+            const float off = static_cast<float>(above) - rough_above(b), want = static_cast<float>(want_mass);
+            b = min(max(find_bin([&](int, float m, float) { return m + off >= want; }, nullptr), b_lo), b_hi);
             continue;
           }
-          want_mass = above * (1.0 + 1e-15);
-        }
-        if (!counting && above + in < want_mass && moved >= 0 && b + 1 < kBins) {
-          moved = 1;
-          ++b;
-          continue;
+          if (higher) {  // sums of the same values in two groupings contradict one another in their last places: the bin before is kept whole
+            --b;
+            b_lo = b_hi = b;
+            want_mass = 1e300;
+            continue;
+          }
+          if (lower) want_mass = 1e300;
         }
         if (in_n == 0) return;  // all of them stay
         // While they are too many for one CTA: halved by value.
@@ -606,12 +597,11 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
             const int index = cand_index[i];
             int better = 0;
             for (int j = 0; j < m; ++j) better += cand_key[j] > key || (cand_key[j] == key && cand_index[j] < index) ? 1 : 0;
-            // by rank, into the bins' place: they are no longer needed by this CTA once the edge is known
             if (counting ? above_n + better + 1 == want_count : false) {
               edge_s.key = key;
               edge_s.index = index;
             }
-            if (!counting) reinterpret_cast<int*>(bin_mass)[better] = i;
+            if (!counting) s_order[better] = i;
           }
           __syncthreads();
           if (!counting && warp == 0) {  // running sums by rank, 32 at a time
@@ -619,7 +609,7 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
             int last = 0;
             bool over = false;
             for (int j0 = 0; j0 < m && !over; j0 += 32) {
-              const int at = j0 + lane < m ? reinterpret_cast<int*>(bin_mass)[j0 + lane] : 0;
+              const int at = j0 + lane < m ? s_order[j0 + lane] : 0;
               const double w = j0 + lane < m ? weight(ValueOf(cand_key[at])) : 0.0;
               double up = w;
 #pragma unroll
@@ -636,7 +626,7 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
               run += __shfl_sync(0xffffffffu, up, 31);
             }
             if (lane == 0) {
-              const int at = reinterpret_cast<int*>(bin_mass)[last];
+              const int at = s_order[last];
               edge_s.key = cand_key[at];
               edge_s.index = cand_index[at];
             }
@@ -658,21 +648,20 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
     };
     double mass = all;
     if (by_k) {
-      const int b = find_bin([&](int c, float) { return c >= top_k; }, nullptr);
+      const int b = find_bin([&](int c, float, float) { return c >= top_k; }, nullptr);
       find_edge(b, true, top_k, 0.0, 0u, a.n, by_p ? &mass : nullptr);
     }
     if (by_p) {
       const double share = fmax(static_cast<double>(top_p) * mass, 1e-300);  // above 0: the first one stays
-      const float rough = static_cast<float>(share);
+      const float rough = static_cast<float>(share), part_of = fmaxf(top_p, 0.f);
       const int last = by_k ? bin_of(ValueOf(edge_key)) : kBins - 1;
-      const int b = min(find_bin([&](int, float m) { return m >= rough; }, nullptr), last);
+      const int b = min(find_bin([&](int, float m, float total) { return m >= (by_k ? rough : part_of * total); }, nullptr), last);
       double unused;
       find_edge(b, false, 0, share, edge_key, edge_index, &unused);
     }
   }
 
   // 4: what is kept, by warp, in index order.
-  const double least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
   const bool whole = edge_key == 0u;
   auto kept = [&](int i, float f) -> double {  // the weight of a kept value, 0 of others
     if (!whole) {
@@ -680,14 +669,15 @@ __global__ void __launch_bounds__(kSampleThreads) SampleKernel(const __grid_cons
       if (key < edge_key || (key == edge_key && lo + i > edge_index)) return 0.0;
     }
     const double w = weight(f);
-    return w < least ? 0.0 : w;
+    return least > 0.0 && w < least ? 0.0 : w;
   };
-  double mine = 0.0;
+  double mine = above_bin >= 0 ? above_mine : 0.0;
   for (int i = w_lo + lane * kVec; i < w_hi; i += 32 * kVec) {
     float f[kVec];
     values(i, w_hi, f);
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) mine += kept(i + k, f[k]);
+    for (int k = 0; k < kVec; ++k)
+      if (above_bin < 0 || bin_of(f[k]) == above_bin) mine += kept(i + k, f[k]);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
