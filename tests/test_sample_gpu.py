@@ -110,6 +110,18 @@ def test_masked_infinite_and_missing_values(setting):
     check(x, u, **setting)
 
 
+@pytest.mark.parametrize("n", [4000, 40000])
+@pytest.mark.parametrize("setting", [dict(), dict(top_k=700), dict(top_k=3000), dict(top_p=0.5), dict(top_k=2000, top_p=0.7), dict(min_p=0.1), dict(temperature=float("inf"), top_p=0.9)])
+def test_many_infinities(setting, n):
+    """More of them than one CTA ranks, beside values that then weigh nothing."""
+    x, u = rows_of(4, n, seed=n)
+    x[0, ::3] = float("inf")
+    x[1, 5:] = float("inf")
+    x[2] = float("inf")
+    x[3, 1::2] = torch.finfo(torch.float32).max
+    check(x, u, **setting)
+
+
 @pytest.mark.parametrize("setting", [dict(), dict(top_k=5), dict(top_p=0.5), dict(temperature=1e30), dict(temperature=1e-30)])
 def test_random_numbers_at_their_ends(setting):
     x, _ = rows_of(8, 1000, seed=7)
@@ -124,6 +136,16 @@ def test_row_counts(rows):
         assert ops.sample(x, u).shape == (0,)
     else:
         check(x, u, top_k=30, top_p=0.9)
+
+
+@pytest.mark.parametrize("top_k", [600, 1000, 5000])
+@pytest.mark.parametrize("top_p", [0.5, 0.95, 0.999])
+def test_few_tokens_above_many(top_p, top_k):
+    """Rows whose first tokens outweigh thousands of others, cut deep among those."""
+    x, u = rows_of(16, 32768, seed=5, spread=2.0)
+    x[:, 100:108] += 12.0
+    check(x, u, top_k=top_k, top_p=top_p)
+    check(x, u, top_p=top_p, temperature=1.4)
 
 
 def test_borders_fall_where_64_bits_have_them():

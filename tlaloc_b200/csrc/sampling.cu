@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
     cluster.sync();
     for (int q = 0; q < ranks; ++q) best = max(best, told_key[q]);
   }
-  const float top = ValueOf(best);
+  float top = ValueOf(best);
   const int chunk = ((n + kSampleWarps - 1) / kSampleWarps + 31) / 32 * 32;  // a warp's stretch of the part: whole 16-byte words
   const int w_lo = min(warp * chunk, n), w_hi = min(w_lo + chunk, n);
 
@@ -192,14 +192,20 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
     return;
   }
 
-  const double scale = 1.4426950408889634074 / static_cast<double>(temperature), dtop = static_cast<double>(top);
+  // Where the largest is +infinity all but these weigh nothing: they are looked at as 0 and the others as -infinity.
   const bool infinite = top == INFINITY;
-  // Values from here down (and NaN) weigh nothing: 2^-1000, or anything beside infinity.
+  if (infinite) top = 0.f;
+  const double scale = 1.4426950408889634074 / static_cast<double>(temperature), dtop = static_cast<double>(top);
+  // Values from here down (and NaN) weigh nothing: 2^-1000.  Always below the largest.
   const double low = dtop - 1000.0 / scale;
-  const float cut = infinite ? top : low < -3.4028234663852886e38 ? -INFINITY : static_cast<float>(low);
+  const float cut = low < -3.4028234663852886e38 ? -INFINITY : fminf(static_cast<float>(low), ValueOf(KeyOf(top) - 1));
   auto weight = [&](float f) -> double {  // 1 for the largest: 2^0 is exact
     const double w = TableExp2((static_cast<double>(f) - dtop) * scale, table);
-    return f > cut ? w : f == top ? 1.0 : 0.0;
+    return f > cut ? w : 0.0;
+  };
+  auto value_at = [&](int i) {
+    const float f = ToF32(v[i]);
+    return !infinite ? f : f == INFINITY ? 0.f : -INFINITY;
   };
   // A lane's values [i, i + kVec) of the part, -infinity behind its end.
   constexpr int kVec = 16 / static_cast<int>(sizeof(XT));
@@ -208,10 +214,19 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
       const uint4 raw = *reinterpret_cast<const uint4*>(part + i);  // the part's end is padded to whole words
       const XT* e = reinterpret_cast<const XT*>(&raw);
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) f[k] = i + k < end ? ToF32(e[k]) : -INFINITY;
+      for (int k = 0; k < kVec; ++k) f[k] = ToF32(e[k]);
+      if (i + kVec > end) {
+#pragma unroll
+        for (int k = 0; k < kVec; ++k)
+          if (i + k >= end) f[k] = -INFINITY;
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < kVec; ++k) f[k] = i + k < end ? ToF32(x[i + k]) : -INFINITY;
+    }
+    if (infinite) {
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) f[k] = f[k] == INFINITY ? 0.f : -INFINITY;
     }
   };
   auto each = [&](auto&& work) {  // work(place in the part, value), every place of it
@@ -226,8 +241,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
   // The bin of a value: a function that does not rise with it, however it is rounded.
   const float fscale = fminf(static_cast<float>(scale) * kBinsPerOctave, 3.0e38f);
   auto bin_of = [&](float f) -> int {
-    if (f == top) return 0;
-    if (!(f > -INFINITY) || top == INFINITY) return kBins - 1;
+    if (!(f > -INFINITY)) return kBins - 1;
     return static_cast<int>(fminf((top - f) * fscale, static_cast<float>(kBins - 1)));
   };
 
@@ -541,7 +555,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
           }
           // The index of the quota-th of them: equal ones of the ranks before, of the warps before, then by 32.
           int equal = 0;
-          for (int i = w_lo + lane; i < w_hi; i += 32) equal += KeyOf(ToF32(v[i])) == key ? 1 : 0;
+          for (int i = w_lo + lane; i < w_hi; i += 32) equal += KeyOf(value_at(i)) == key ? 1 : 0;
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) equal += __shfl_xor_sync(0xffffffffu, equal, o);
           __syncthreads();
@@ -560,7 +574,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
           if (before < quota && before + equal >= quota) {
             int seen = before;
             for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
-              const bool is = i0 + lane < w_hi && KeyOf(ToF32(v[i0 + lane])) == key;
+              const bool is = i0 + lane < w_hi && KeyOf(value_at(i0 + lane)) == key;
               const unsigned ties = __ballot_sync(0xffffffffu, is);
               if (is && seen + __popc(ties & ((1u << lane) - 1u)) + 1 == quota) {
                 for (int q = 0; q < ranks; ++q) cluster.map_shared_rank(&edge_s, q)->index = lo + i0 + lane;
@@ -672,6 +686,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
     return least > 0.0 && w < least ? 0.0 : w;
   };
   double mine = above_bin >= 0 ? above_mine : 0.0;
+  if (whole && least == 0.0) {
+    for (int i = w_lo + lane * kVec; i < w_hi; i += 32 * kVec) {
+      float f[kVec];
+      values(i, w_hi, f);
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) mine += weight(f[k]);
+    }
+  } else
   for (int i = w_lo + lane * kVec; i < w_hi; i += 32 * kVec) {
     float f[kVec];
     values(i, w_hi, f);
