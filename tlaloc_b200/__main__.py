@@ -2,6 +2,7 @@
 
     python -m tlaloc_b200 models
     python -m tlaloc_b200 generate --model DIR --max-new 32 --prompt 5,17,3 --prompt 9,9,1
+    python -m tlaloc_b200 generate --model DIR --prompt 5,17,3 --temperature 0.8 --top-k 50 --top-p 0.95 --seed 7
     python -m tlaloc_b200 trace --model DIR --dtype float32 --out DIR --max-tokens 4096 < steps
 """
 from __future__ import annotations
@@ -12,7 +13,7 @@ import sys
 
 
 def generate(argv) -> int:
-    ap = argparse.ArgumentParser(prog="tlaloc_b200 generate", description="greedy continuations of token-id prompts")
+    ap = argparse.ArgumentParser(prog="tlaloc_b200 generate", description="continuations of token-id prompts, greedy unless a temperature is given")
     ap.add_argument("--model", required=True, help="folder with config.json and .safetensors weights")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     ap.add_argument("--prompt", action="append", default=[], help="token ids with commas between them; may be repeated")
@@ -21,11 +22,22 @@ def generate(argv) -> int:
     ap.add_argument("--stop", type=int, action="append", default=[], help="a token id that ends a continuation")
     ap.add_argument("--max-len", type=int, default=4096, help="longest sequence, prompt and continuation")
     ap.add_argument("--cache-tokens", type=int, help="tokens the cache holds (default: four sequences of --max-len)")
+    ap.add_argument("--temperature", type=float, default=0.0, help="0 (the default): greedy")
+    ap.add_argument("--top-k", type=int, default=0, help="draw among this many tokens (0: all)")
+    ap.add_argument("--top-p", type=float, default=1.0, help="draw among the first tokens that hold this share of the probability")
+    ap.add_argument("--min-p", type=float, default=0.0, help="draw among tokens at least this likely beside the likeliest one")
+    ap.add_argument("--seed", type=int, default=0, help="prompt i draws with seed + i")
     args = ap.parse_args(argv)
     import torch
 
     from . import registry
     from .engine import Engine
+    from .sampling import Sampling
+
+    try:
+        sampling = Sampling(args.temperature, args.top_k, args.top_p, args.min_p, args.seed)
+    except ValueError as e:
+        ap.error(str(e))
 
     prompts = [[int(t) for t in p.split(",")] for p in args.prompt]
     if args.prompts:
@@ -34,7 +46,7 @@ def generate(argv) -> int:
     if not prompts:
         ap.error("no prompt")
     engine = Engine(registry.load(args.model, dtype=getattr(torch, args.dtype), max_len=args.max_len, cache_tokens=args.cache_tokens))
-    for out in engine.generate(prompts, args.max_new, args.stop):
+    for out in engine.generate(prompts, args.max_new, args.stop, sampling if args.temperature > 0 else None):
         print(json.dumps(out))
     return 0
 

@@ -372,6 +372,11 @@ class Decoder(StepModel):
             return self.logits[torch.as_tensor(want, dtype=torch.long, device=self.device)]
         return ops.embedding(self.logits, self.want_rows[:len(rows)]) if len(rows) else self.logits[:0]
 
+    def sample(self, logits: torch.Tensor, draws) -> torch.Tensor:
+        if self.world > 1:
+            raise NotImplementedError("under tensor parallelism each rank has its part of the vocabulary's logits: only greedy tokens are merged over ranks")
+        return super().sample(logits, draws)
+
     # ------------------------------------------------------------------ traffic model
 
     def step_bytes(self, seq_lens: np.ndarray) -> dict:

@@ -1,13 +1,16 @@
-"""Serving over one model: sequences that are fed tokens step by step, and greedy generation of many requests.
+"""Serving over one model: sequences that are fed tokens step by step, and generation of many requests, greedy or sampled.
 
 Both run the model's one step function over the same paged cache: `Engine.feed` for a caller that brings the tokens, `Engine.generate` with
 the scheduler choosing them.
 """
 from __future__ import annotations
 
+from dataclasses import replace
+
 import torch
 
 from .paging import PagePool, Sequence, stage_ragged
+from .sampling import Sampling
 from .scheduler import Request, Scheduler
 from .step_model import StepModel
 
@@ -70,16 +73,26 @@ class Engine:
         logits = self._run([(r.seq, tokens) for r, tokens in work], want)
         done = []
         if want:
-            for r, token in zip(ends, self.model.greedy(logits).tolist()):
+            if any(r.sampling is not None for r in ends):
+                tokens = self.model.sample(logits, [(r.sampling, len(r.output)) for r in ends])
+            else:
+                tokens = self.model.greedy(logits)
+            for r, token in zip(ends, tokens.tolist()):
                 r.output.append(int(token))
                 if r.finished:
                     self.scheduler.finish(r)
                     done.append(r)
         return done
 
-    def generate(self, prompts, max_new: int, stop=()) -> list[list[int]]:
-        """Greedy continuations of `prompts` (lists of token ids), `max_new` tokens each or up to a stop token."""
-        requests = [Request(i, list(p), max_new, frozenset(stop)) for i, p in enumerate(prompts)]
+    def generate(self, prompts, max_new: int, stop=(), sampling=None) -> list[list[int]]:
+        """Continuations of `prompts` (lists of token ids), `max_new` tokens each or up to a stop token.  sampling: None for greedy ones, a `Sampling`
+        for all (prompt i draws with its seed + i) or a list of one (or None) per prompt."""
+        prompts = list(prompts)
+        if sampling is None or isinstance(sampling, Sampling):
+            sampling = [sampling and replace(sampling, seed=(sampling.seed + i) % 2**64) for i in range(len(prompts))]
+        elif len(sampling) != len(prompts):
+            raise ValueError(f"{len(sampling)} sampling settings for {len(prompts)} prompts")
+        requests = [Request(i, list(p), max_new, frozenset(stop), sampling=s) for i, (p, s) in enumerate(zip(prompts, sampling))]
         for r in requests:
             if not r.prompt or len(r.prompt) + max_new > self.model.max_blocks * self.model.block_size:
                 raise ValueError(f"prompt {r.id}: {len(r.prompt)} + {max_new} tokens; this engine takes 1 to "

@@ -5,6 +5,7 @@ from collections import deque
 from dataclasses import dataclass, field
 
 from .paging import PagePool, Sequence
+from .sampling import Sampling
 
 
 @dataclass
@@ -15,6 +16,7 @@ class Request:
     stop: frozenset = frozenset()
     output: list[int] = field(default_factory=list)
     seq: Sequence = field(default_factory=Sequence)
+    sampling: Sampling | None = None  # None: the first maximum
 
     @property
     def tokens(self) -> list[int]:

@@ -12,6 +12,7 @@ import torch
 
 from . import _native as N
 from . import ops
+from . import sampling
 from .paging import PADDING_LENGTH, PADDING_PAGE, PADDING_SLOT, PADDING_STATE, RaggedStep
 
 
@@ -148,6 +149,12 @@ class StepModel:
     def greedy(self, logits: torch.Tensor) -> torch.Tensor:
         """First maximum of every row of logits, int32 on the device."""
         return ops.argmax(logits)
+
+    def sample(self, logits: torch.Tensor, draws) -> torch.Tensor:
+        """A token for every row of logits, drawn as draws [(Sampling or None, index of the draw)] say, int32 on the device."""
+        packed = torch.from_numpy(sampling.pack(draws)).to(logits.device)
+        uniforms, temperature, top_p, min_p = packed[:4].view(torch.float32)
+        return ops.sample(logits, uniforms, temperature=temperature, top_k=packed[4], top_p=top_p, min_p=min_p)
 
     def _padded(self, step: RaggedStep, rows: int):
         """The step's inputs with every row carrying its own block table, padded to `rows` rows: slot -1, length 1, page 0."""
