@@ -148,6 +148,31 @@ def test_few_tokens_above_many(top_p, top_k):
     check(x, u, top_p=top_p, temperature=1.4)
 
 
+@pytest.mark.parametrize("n", [4099, 50257, 128256])
+@pytest.mark.parametrize("spread", [0.02, 0.3, 1.0])
+@pytest.mark.parametrize("step", [None, 0.001, 0.05])
+def test_flat_rows(spread, step, n):
+    """Edges among thousands of values that lie close together, or are equal."""
+    x, u = rows_of(12, n, seed=n, spread=spread)
+    if step is not None:
+        x = (x / step).round() * step
+    p = torch.tensor([0.0, 0.01, 0.1, 0.3, 0.5, 0.7, 0.9, 0.97, 0.99, 0.999, 0.9999, 0.99999], device="cuda")
+    k = torch.tensor([600, 1000, n // 8, n // 4, n // 2, n // 2 + 1, n * 3 // 4, n - 700, n - 1, n, 0, 3000], dtype=torch.int32, device="cuda")
+    check(x, u, top_p=p)
+    check(x, u, top_k=k)
+    check(x, u, top_p=p, top_k=k.flip(0), min_p=0.5)
+    check(x, u, top_p=p, top_k=k, temperature=0.3)
+
+
+@pytest.mark.parametrize("share", [0.9906, 0.9914, 0.9922, 0.9999, 1.0 - 2.0**-24])
+def test_values_at_the_ends_of_what_masses_are_guessed_by(share):
+    """Two million values just below borders of a 8192nd of an octave, an edge among the scattered ones behind them."""
+    part = np.log(2.0) / 8192
+    x = np.concatenate([-np.repeat(np.arange(400) * part * (1 + 1e-6), 5000), -(400 + 112 * np.random.RandomState(1).rand(33600)) * part, [-30.0]])
+    x = torch.from_numpy(np.random.RandomState(2).permutation(x)).float().cuda().repeat(2, 1)
+    check(x, torch.tensor([0.25, 1 - 2.0**-24], device="cuda"), top_p=share)
+
+
 def test_borders_fall_where_64_bits_have_them():
     """Flat rows over the largest vocabulary: a border between tokens every 4e-6, so that sums of f32 would miss many draws."""
     x, u = rows_of(256, 262144, seed=8, spread=0.5)

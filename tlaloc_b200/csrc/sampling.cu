@@ -48,6 +48,8 @@ constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kBins = 1024, kMaxRanks = 8;
 constexpr float kBinsPerOctave = 16.f;  // of w: the last bin begins 64 octaves below the largest
 constexpr int kRanked = 512;            // values of a bin that one CTA ranks
+constexpr int kSubs = 512;              // parts of a bin with more values
+constexpr int kBeside = 32;             // values on either side of where rough masses put an edge that are ranked with it
 
 // Values in an order of unsigned numbers: -0 as 0, NaN as -infinity (never drawn).
 __device__ __forceinline__ uint32_t KeyOf(float x)
@@ -92,6 +94,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
   __shared__ struct {
     uint32_t key;
     int index;
+    bool inside;
   } edge_s;
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank()), ranks = static_cast<int>(cluster.num_blocks());
@@ -263,19 +266,23 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
       if (by_p) all += weight(f);
     });
     if (by_p) all = cluster_sum(all, red, told_mass);
-    if (ranks > 1) {  // the row's bins: every rank adds up an equal share of them over all ranks and tells everyone
+    // Counts over all ranks, in each: every rank adds up an equal share of them and tells everyone.
+    auto add_over_ranks = [&](int* counts, int size) {
+      if (ranks == 1) {
+        __syncthreads();
+        return;
+      }
       cluster.sync();
-      const int share = kBins / ranks, b = rank * share + tid;
+      const int share = size / ranks, i = rank * share + tid;
       int c = 0;
       if (tid < share)
-        for (int q = 0; q < ranks; ++q) c += *cluster.map_shared_rank(bin_count + b, q);
+        for (int q = 0; q < ranks; ++q) c += *cluster.map_shared_rank(counts + i, q);
       cluster.sync();
       if (tid < share)
-        for (int q = 0; q < ranks; ++q) *cluster.map_shared_rank(bin_count + b, q) = c;
+        for (int q = 0; q < ranks; ++q) *cluster.map_shared_rank(counts + i, q) = c;
       cluster.sync();
-    } else {
-      __syncthreads();
-    }
+    };
+    add_over_ranks(bin_count, kBins);
     // The first bin at whose end `enough(count, rough mass, rough mass of all)` holds, the last one if it never does; *upto: the count there.
     auto find_bin = [&](auto&& enough, int* upto) {
       __shared__ int found_s, upto_s;
@@ -419,10 +426,34 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
     };
     // Four sums at once.
     auto cluster_sums = [&](int& c0, int& c1, double& m0, double& m1) {
-      c0 = block_sum(c0, ired);
-      c1 = block_sum(c1, ired);
-      m0 = block_sum(m0, red);
-      m1 = block_sum(m1, red);
+      __shared__ int cs[2][kSampleWarps];
+      __shared__ double ms[2][kSampleWarps];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        c0 += __shfl_xor_sync(0xffffffffu, c0, o);
+        c1 += __shfl_xor_sync(0xffffffffu, c1, o);
+        m0 += __shfl_xor_sync(0xffffffffu, m0, o);
+        m1 += __shfl_xor_sync(0xffffffffu, m1, o);
+      }
+      __syncthreads();
+      if (lane == 0) {
+        cs[0][warp] = c0;
+        cs[1][warp] = c1;
+        ms[0][warp] = m0;
+        ms[1][warp] = m1;
+      }
+      __syncthreads();
+      c0 = c1 = 0;
+      m0 = m1 = 0.0;
+      if (ranks == 1 || tid < ranks) {
+#pragma unroll
+        for (int w = 0; w < kSampleWarps; ++w) {
+          c0 += cs[0][w];
+          c1 += cs[1][w];
+          m0 += ms[0][w];
+          m1 += ms[1][w];
+        }
+      }
       if (ranks == 1) return;
       if (tid < ranks) {
         *cluster.map_shared_rank(told_counts[0] + rank, tid) = c0;
@@ -462,6 +493,63 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
       most_key = range_s[1];
       __syncthreads();
     };
+    // The part of bin b that a value of it lies in: does not rise with it either.  Without a fused multiply-add, so that counting and gathering agree on it.
+    int* const sub_count = reinterpret_cast<int*>(s_weight);
+    auto sub_of = [&](float f, int b) -> int {
+      if (!(f > -INFINITY)) return kSubs - 1;
+      return static_cast<int>(fminf(fmaxf(__fsub_rn(__fmul_rn(top - f, fscale), static_cast<float>(b)), 0.f) * kSubs, static_cast<float>(kSubs - 1)));
+    };
+    // Parts [*s_lo, *s_hi] of bin b, whose part `tid` has c values: the one that holds the want_count-th, or those around the one where the rough mass reaches `want`.
+    // *before, *among: how many values lie in the parts before and in these.  False where they are none, or more than kRanked.
+    auto find_sub = [&](int c, int b, int want_count, float want, bool counting, int* s_lo, int* s_hi, int* before, int* among) {
+      __shared__ int cs[kSampleWarps], found_s, lo_s, hi_s, at_s[2], edge_n[2];
+      __shared__ float ms[kSampleWarps];
+      const float m = static_cast<float>(c) * exp2f(-(static_cast<float>(b) + (static_cast<float>(tid) + 0.5f) / kSubs) / kBinsPerOctave);
+      int cu = c;
+      float mu = m;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int cc = __shfl_up_sync(0xffffffffu, cu, o);
+        const float mm = __shfl_up_sync(0xffffffffu, mu, o);
+        if (lane >= o) {
+          cu += cc;
+          mu += mm;
+        }
+      }
+      if (lane == 31) {
+        cs[warp] = cu;
+        ms[warp] = mu;
+      }
+      if (tid == 0) {
+        found_s = lo_s = kSubs - 1;
+        hi_s = 0;
+      }
+      __syncthreads();
+      for (int w = 0; w < warp; ++w) {
+        cu += cs[w];
+        mu += ms[w];
+      }
+      if (counting ? cu >= want_count : mu >= want) atomicMin(&found_s, tid);
+      __syncthreads();
+      if (tid == found_s) {
+        at_s[0] = cu - c;
+        at_s[1] = cu;
+      }
+      __syncthreads();
+      const int beside = counting ? 0 : max(min((kRanked - (at_s[1] - at_s[0])) / 2, kBeside), 0);
+      if (tid == found_s || (tid < found_s && at_s[0] - (cu - c) <= beside)) atomicMin(&lo_s, tid);
+      if (tid == found_s || (tid > found_s && cu - at_s[1] <= beside)) atomicMax(&hi_s, tid);
+      __syncthreads();
+      if (tid == lo_s) edge_n[0] = cu - c;
+      if (tid == hi_s) edge_n[1] = cu;
+      __syncthreads();
+      *s_lo = lo_s;
+      *s_hi = hi_s;
+      *before = edge_n[0];
+      *among = edge_n[1] - edge_n[0];
+      __syncthreads();
+      return *among > 0 && *among <= kRanked;  // none: the rough masses end short of the last values
+    };
     // The edge in or next to bin `b`.  Counting: the value of rank `want_count`.  Otherwise: the last value whose betters hold less than `want_mass`, none beyond
     // (limit_key, limit_index).  kept_mass, if given: the exact mass of what is kept.
     auto find_edge = [&](int b, bool counting, int want_count, double want_mass, uint32_t limit_key, int limit_index, double* kept_mass) {
@@ -470,8 +558,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
         // Exactly what lies above the bin, and in it.
         int above_n = 0, in_n = 0;
         double above = 0.0, in = 0.0;
-        uint32_t k_lo = 0xffffffffu, k_hi = 0;  // the bin's values lie between these keys
         above_mine = 0.0;
+        static_assert(kSubs == kSampleThreads, "a thread a part");
+        sub_count[tid] = 0;
+        __syncthreads();
         for (int i0 = w_lo + lane * kVec; i0 < w_hi; i0 += 32 * kVec) {
           float f[kVec];
           values(i0, w_hi, f);
@@ -488,13 +578,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
             } else if (key > limit_key || (key == limit_key && lo + i <= limit_index)) {
               ++in_n;
               if (!counting) in += weight(f[k]);
-              k_lo = min(k_lo, key);
-              k_hi = max(k_hi, key);
+              atomicAdd(&sub_count[sub_of(f[k], b)], 1);
             }
           }
         }
         above_bin = counting ? -1 : b;
-        cluster_range(k_lo, k_hi);
         cluster_sums(above_n, in_n, above, in);
         if (!counting) {
           // The edge lies higher or lower: the exact mass above this bin says by how much the rough ones are off.
@@ -515,149 +603,205 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
           if (lower) want_mass = 1e300;
         }
         if (in_n == 0) return;  // all of them stay
-        // While they are too many for one CTA: halved by value.
-        while (in_n > kRanked && k_lo < k_hi) {
-          const uint32_t mid = k_lo + (k_hi - k_lo) / 2;  // the upper half: keys above it
-          int up_n = 0;
-          double up = 0.0;
-          each([&](int i, float f) {
-            const uint32_t key = KeyOf(f);
-            if (key <= mid || key > k_hi || bin_of(f) != b || key < limit_key || (key == limit_key && lo + i > limit_index)) return;
-            ++up_n;
-            if (!counting) up += weight(f);
-          });
-          int none_n = 0;
-          double none = 0.0;
-          cluster_sums(up_n, none_n, up, none);
-          // Neither half is taken empty.
-          const bool higher = up_n > 0 && (up_n == in_n || (counting ? above_n + up_n >= want_count : above + up >= want_mass));
-          if (higher) {
-            k_lo = mid + 1;
-            in_n = up_n;
+        // The bin's values that are ranked: between these keys, in these parts of it.
+        uint32_t k_lo = 0u, k_hi = 0xffffffffu;
+        int s_lo = 0, s_hi = kSubs - 1;
+        bool to_end = true;  // they reach down to the bin's last one
+        const int bin_above_n = above_n, bin_n = in_n;
+        const double bin_above = above;
+        bool by_subs = false;
+        int upto = 0;
+        if (in_n > kRanked) {
+          // Too many for one CTA: those in the part where the edge must lie, by their exact counts, or the few around the place that their rough masses give.
+          add_over_ranks(sub_count, kSubs);
+          const int c = sub_count[tid];
+          by_subs = find_sub(c, b, counting ? want_count - above_n : 0, counting ? 0.f : static_cast<float>(fmin(want_mass - above, 3e38)), counting, &s_lo, &s_hi, &upto, &in_n);
+          if (by_subs) {
+            to_end = upto + in_n == bin_n;
+            if (counting) above_n += upto;
           } else {
-            k_hi = mid;
-            in_n -= up_n;
-            above_n += up_n;
-            above += up;
+            s_lo = 0;
+            s_hi = kSubs - 1;
+            in_n = bin_n;
           }
         }
-        if (in_n > kRanked) {  // that many equal values: the edge is one of them, by how many there is room for
-          const uint32_t key = k_lo;
-          const double w = weight(ValueOf(key));
-          int quota = in_n;
-          if (counting) {
-            quota = want_count - above_n;
-          } else if (w > 0.0) {  // the j-th stays while above + j w < want
-            double most = ceil((want_mass - above) / w);
-            if (most > 1.0 && above + (most - 1.0) * w >= want_mass) most -= 1.0;
-            if (above + most * w < want_mass) most += 1.0;
-            quota = static_cast<int>(fmin(static_cast<double>(in_n), fmax(most, 1.0)));
+        for (;; by_subs = false) {
+          // Where that finds none few enough, or missed: the bin is halved by value while it holds too many.
+          if (in_n > kRanked) {
+            k_lo = 0xffffffffu;
+            k_hi = 0u;
+            each([&](int i, float f) {
+              const uint32_t key = KeyOf(f);
+              if (bin_of(f) != b || key < limit_key || (key == limit_key && lo + i > limit_index)) return;
+              k_lo = min(k_lo, key);
+              k_hi = max(k_hi, key);
+            });
+            cluster_range(k_lo, k_hi);
           }
-          // The index of the quota-th of them: equal ones of the ranks before, of the warps before, then by 32.
-          int equal = 0;
-          for (int i = w_lo + lane; i < w_hi; i += 32) equal += KeyOf(value_at(i)) == key ? 1 : 0;
+          while (in_n > kRanked && k_lo < k_hi) {
+            const uint32_t mid = k_lo + (k_hi - k_lo) / 2;  // the upper half: keys above it
+            int up_n = 0;
+            double up = 0.0;
+            each([&](int i, float f) {
+              const uint32_t key = KeyOf(f);
+              if (key <= mid || key > k_hi || bin_of(f) != b || key < limit_key || (key == limit_key && lo + i > limit_index)) return;
+              ++up_n;
+              if (!counting) up += weight(f);
+            });
+            int none_n = 0;
+            double none = 0.0;
+            cluster_sums(up_n, none_n, up, none);
+            // Neither half is taken empty.
+            const bool higher = up_n > 0 && (up_n == in_n || (counting ? above_n + up_n >= want_count : above + up >= want_mass));
+            if (higher) {
+              k_lo = mid + 1;
+              in_n = up_n;
+            } else {
+              k_hi = mid;
+              in_n -= up_n;
+              above_n += up_n;
+              above += up;
+            }
+          }
+          if (in_n > kRanked) {  // that many equal values: the edge is one of them, by how many there is room for
+            const uint32_t key = k_lo;
+            const double w = weight(ValueOf(key));
+            int quota = in_n;
+            if (counting) {
+              quota = want_count - above_n;
+            } else if (w > 0.0) {  // the j-th stays while above + j w < want
+              double most = ceil((want_mass - above) / w);
+              if (most > 1.0 && above + (most - 1.0) * w >= want_mass) most -= 1.0;
+              if (above + most * w < want_mass) most += 1.0;
+              quota = static_cast<int>(fmin(static_cast<double>(in_n), fmax(most, 1.0)));
+            }
+            // The index of the quota-th of them: equal ones of the ranks before, of the warps before, then by 32.
+            int equal = 0;
+            for (int i = w_lo + lane; i < w_hi; i += 32) equal += KeyOf(value_at(i)) == key ? 1 : 0;
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) equal += __shfl_xor_sync(0xffffffffu, equal, o);
-          __syncthreads();
-          if (lane == 0) ired[warp] = equal;
-          __syncthreads();
-          int before = 0, mine = 0;
-          for (int w2 = 0; w2 < kSampleWarps; ++w2) {
-            if (w2 < warp) before += ired[w2];
-            mine += ired[w2];
-          }
-          if (ranks > 1) {
-            if (tid < ranks) *cluster.map_shared_rank(told_count + rank, tid) = mine;
-            cluster.sync();
-            for (int q = 0; q < rank; ++q) before += told_count[q];
-          }
-          if (before < quota && before + equal >= quota) {
-            int seen = before;
-            for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
-              const bool is = i0 + lane < w_hi && KeyOf(value_at(i0 + lane)) == key;
-              const unsigned ties = __ballot_sync(0xffffffffu, is);
-              if (is && seen + __popc(ties & ((1u << lane) - 1u)) + 1 == quota) {
-                for (int q = 0; q < ranks; ++q) cluster.map_shared_rank(&edge_s, q)->index = lo + i0 + lane;
+            for (int o = 16; o > 0; o >>= 1) equal += __shfl_xor_sync(0xffffffffu, equal, o);
+            __syncthreads();
+            if (lane == 0) ired[warp] = equal;
+            __syncthreads();
+            int before = 0, mine = 0;
+            for (int w2 = 0; w2 < kSampleWarps; ++w2) {
+              if (w2 < warp) before += ired[w2];
+              mine += ired[w2];
+            }
+            if (ranks > 1) {
+              if (tid < ranks) *cluster.map_shared_rank(told_count + rank, tid) = mine;
+              cluster.sync();
+              for (int q = 0; q < rank; ++q) before += told_count[q];
+            }
+            if (before < quota && before + equal >= quota) {
+              int seen = before;
+              for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
+                const bool is = i0 + lane < w_hi && KeyOf(value_at(i0 + lane)) == key;
+                const unsigned ties = __ballot_sync(0xffffffffu, is);
+                if (is && seen + __popc(ties & ((1u << lane) - 1u)) + 1 == quota) {
+                  for (int q = 0; q < ranks; ++q) cluster.map_shared_rank(&edge_s, q)->index = lo + i0 + lane;
+                }
+                seen += __popc(ties);
               }
-              seen += __popc(ties);
+            }
+            cluster.sync();
+            edge_key = key;
+            edge_index = edge_s.index;
+            cluster.sync();
+            if (kept_mass != nullptr) *kept_mass = mass_upto_edge();
+            return;
+          }
+          // The values of the bin (or of what is left of it) in rank 0, in any order.
+          if (tid == 0) cand_n = 0;
+          cluster.sync();
+          int* const count0 = cluster.map_shared_rank(&cand_n, 0);
+          uint32_t* const key0 = cluster.map_shared_rank(cand_key, 0);
+          int* const index0 = cluster.map_shared_rank(cand_index, 0);
+          double more = 0.0;
+          each([&](int i, float f) {
+            const uint32_t key = KeyOf(f);
+            if (bin_of(f) != b || key < k_lo || key > k_hi || key < limit_key || (key == limit_key && lo + i > limit_index)) return;
+            if (by_subs) {
+              const int sub = sub_of(f, b);
+              if (sub < s_lo && !counting) more += weight(f);
+              if (sub < s_lo || sub > s_hi) return;
+            }
+            const int at = atomicAdd(count0, 1);
+            key0[at] = key;
+            index0[at] = lo + i;
+          });
+          if (by_subs && !counting) {
+            above = bin_above + cluster_sum(more, red, told_mass);
+            above_n = bin_above_n + upto;
+          } else {
+            cluster.sync();
+          }
+          if (rank == 0) {
+            // Each value's betters among them, their number and mass: the edge is the one whose betters leave room and which itself takes the last of it.
+            const int m = cand_n;
+            for (int i = tid; i < m; i += kSampleThreads) {
+              const uint32_t key = cand_key[i];
+              const int index = cand_index[i];
+              int better = 0;
+              for (int j = 0; j < m; ++j) better += cand_key[j] > key || (cand_key[j] == key && cand_index[j] < index) ? 1 : 0;
+              if (counting ? above_n + better + 1 == want_count : false) {
+                edge_s.key = key;
+                edge_s.index = index;
+              }
+              if (!counting) s_order[better] = i;
+            }
+            __syncthreads();
+            if (!counting && warp == 0) {  // running sums by rank, 32 at a time
+              double run = above;
+              int last = 0, stayed = 0;
+              bool over = false;
+              for (int j0 = 0; j0 < m && !over; j0 += 32) {
+                const int at = j0 + lane < m ? s_order[j0 + lane] : 0;
+                const double w = j0 + lane < m ? weight(ValueOf(cand_key[at])) : 0.0;
+                double up = w;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                  const double t = __shfl_up_sync(0xffffffffu, up, o);
+                  if (lane >= o) up += t;
+                }
+                double in_front = __shfl_up_sync(0xffffffffu, up, 1);
+                if (lane == 0) in_front = 0.0;
+                const bool stays = j0 + lane < m && (run + in_front < want_mass || (above_n == 0 && j0 + lane == 0));
+                const unsigned stay = __ballot_sync(0xffffffffu, stays);
+                if (stay != 0u) last = j0 + 31 - __clz(stay);
+                over = stay != 0xffffffffu;
+                stayed += __popc(stay);
+                run += __shfl_sync(0xffffffffu, up, 31);
+              }
+              if (lane == 0) {
+                const int at = s_order[last];
+                edge_s.key = cand_key[at];
+                edge_s.index = cand_index[at];
+                edge_s.inside = stayed > 0 && (to_end || stayed < m);
+              }
+            }
+            if (counting && tid == 0) edge_s.inside = true;
+            __syncthreads();
+            if (tid > 0 && tid < ranks) {
+              cluster.map_shared_rank(&edge_s, tid)->key = edge_s.key;
+              cluster.map_shared_rank(&edge_s, tid)->index = edge_s.index;
+              cluster.map_shared_rank(&edge_s, tid)->inside = edge_s.inside;
             }
           }
           cluster.sync();
-          edge_key = key;
+          if (by_subs && !edge_s.inside) {  // the rough masses were that far off
+            above_n = bin_above_n;
+            above = bin_above;
+            in_n = bin_n;
+            to_end = true;
+            cluster.sync();  // read by all
+            continue;
+          }
+          edge_key = edge_s.key;
           edge_index = edge_s.index;
-          cluster.sync();
           if (kept_mass != nullptr) *kept_mass = mass_upto_edge();
           return;
         }
-        // The values of the bin (or of what is left of it) in rank 0, in any order.
-        if (tid == 0) cand_n = 0;
-        cluster.sync();
-        int* const count0 = cluster.map_shared_rank(&cand_n, 0);
-        uint32_t* const key0 = cluster.map_shared_rank(cand_key, 0);
-        int* const index0 = cluster.map_shared_rank(cand_index, 0);
-        each([&](int i, float f) {
-          const uint32_t key = KeyOf(f);
-          if (bin_of(f) != b || key < k_lo || key > k_hi || key < limit_key || (key == limit_key && lo + i > limit_index)) return;
-          const int at = atomicAdd(count0, 1);
-          key0[at] = key;
-          index0[at] = lo + i;
-        });
-        cluster.sync();
-        if (rank == 0) {
-          // Each value's betters among them, their number and mass: the edge is the one whose betters leave room and which itself takes the last of it.
-          const int m = cand_n;
-          for (int i = tid; i < m; i += kSampleThreads) {
-            const uint32_t key = cand_key[i];
-            const int index = cand_index[i];
-            int better = 0;
-            for (int j = 0; j < m; ++j) better += cand_key[j] > key || (cand_key[j] == key && cand_index[j] < index) ? 1 : 0;
-            if (counting ? above_n + better + 1 == want_count : false) {
-              edge_s.key = key;
-              edge_s.index = index;
-            }
-            if (!counting) s_order[better] = i;
-          }
-          __syncthreads();
-          if (!counting && warp == 0) {  // running sums by rank, 32 at a time
-            double run = above;
-            int last = 0;
-            bool over = false;
-            for (int j0 = 0; j0 < m && !over; j0 += 32) {
-              const int at = j0 + lane < m ? s_order[j0 + lane] : 0;
-              const double w = j0 + lane < m ? weight(ValueOf(cand_key[at])) : 0.0;
-              double up = w;
-#pragma unroll
-              for (int o = 1; o < 32; o <<= 1) {
-                const double t = __shfl_up_sync(0xffffffffu, up, o);
-                if (lane >= o) up += t;
-              }
-              double in_front = __shfl_up_sync(0xffffffffu, up, 1);
-              if (lane == 0) in_front = 0.0;
-              const bool stays = j0 + lane < m && (run + in_front < want_mass || (above_n == 0 && j0 + lane == 0));
-              const unsigned stay = __ballot_sync(0xffffffffu, stays);
-              if (stay != 0u) last = j0 + 31 - __clz(stay);
-              over = stay != 0xffffffffu;
-              run += __shfl_sync(0xffffffffu, up, 31);
-            }
-            if (lane == 0) {
-              const int at = s_order[last];
-              edge_s.key = cand_key[at];
-              edge_s.index = cand_index[at];
-            }
-          }
-          __syncthreads();
-          if (tid > 0 && tid < ranks) {
-            cluster.map_shared_rank(&edge_s, tid)->key = edge_s.key;
-            cluster.map_shared_rank(&edge_s, tid)->index = edge_s.index;
-          }
-        }
-        cluster.sync();
-        edge_key = edge_s.key;
-        edge_index = edge_s.index;
-        if (kept_mass != nullptr) {
-          *kept_mass = mass_upto_edge();
-        }
-        return;
       }
     };
     double mass = all;
@@ -670,8 +814,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
       const float rough = static_cast<float>(share), part_of = fmaxf(top_p, 0.f);
       const int last = by_k ? bin_of(ValueOf(edge_key)) : kBins - 1;
       const int b = min(find_bin([&](int, float m, float total) { return m >= (by_k ? rough : part_of * total); }, nullptr), last);
-      double unused;
-      find_edge(b, false, 0, share, edge_key, edge_index, &unused);
+      find_edge(b, false, 0, share, edge_key, edge_index, nullptr);
     }
   }
 
