@@ -75,6 +75,70 @@ __device__ __forceinline__ double TableExp2(double t, const double* table)
   return __hiloint2double(__double2hiint(scaled) + ((k >> 8) << 20), __double2loint(scaled));
 }
 
+// The block's values from the largest down, one a thread, of its first n threads; zeros come last.  No other value twice.  Few are ranked by counting the larger ones of all, more
+// sorted by a bitonic network (strides below 32 through shuffles): 64 values take some 700 cycles counted and 1500 sorted, 512 take 12000 and 3000.
+constexpr int kCounted = 128;
+__device__ __noinline__ uint64_t SortDown(uint64_t v, int n, uint64_t* buffer)
+{
+  const int tid = threadIdx.x;
+  if (tid >= n) v = 0;
+  if (n <= kCounted) {
+    __syncthreads();
+    if (tid < kCounted) {
+      buffer[tid] = v;
+      buffer[kCounted + tid] = 0;
+    }
+    __syncthreads();
+    int larger = 0;
+    if (v != 0) {
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) larger += buffer[j] > v ? 1 : 0;
+      buffer[kCounted + larger] = v;
+    }
+    __syncthreads();
+    return tid < n ? buffer[kCounted + tid] : 0;
+  }
+  for (int k = 2; k < 2 * n; k <<= 1) {
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      uint64_t other;
+      if (j >= 32) {
+        __syncthreads();
+        buffer[tid] = v;
+        __syncthreads();
+        other = buffer[tid ^ j];
+      } else {
+        other = __shfl_xor_sync(0xffffffffu, v, j);
+      }
+      v = ((tid & j) == 0) == ((tid & k) == 0) ? max(v, other) : min(v, other);  // the pair's larger one stays here
+    }
+  }
+  return v;
+}
+
+// The sum of the threads before this one; *all: of all of them.
+__device__ __noinline__ double SumBefore(double w, double* buffer, double* all)
+{
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double up = w;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double t = __shfl_up_sync(0xffffffffu, up, o);
+    if (lane >= o) up += t;
+  }
+  double front = __shfl_up_sync(0xffffffffu, up, 1);
+  if (lane == 0) front = 0.0;
+  __syncthreads();
+  if (lane == 31) buffer[warp] = up;
+  __syncthreads();
+  double run = 0.0, sum = 0.0;
+  for (int q = 0; q < kSampleWarps; ++q) {
+    if (q < warp) run += buffer[q];
+    sum += buffer[q];
+  }
+  *all = sum;
+  return run + front;
+}
+
 template <typename XT>
 __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_constant__ SampleArgs a)
 {
@@ -87,10 +151,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
   __shared__ uint32_t kred[kSampleWarps], told_key[kMaxRanks], range_s[2];
   __shared__ int bin_count[kBins];
   __shared__ double s_weight[kRanked];
-  __shared__ int s_order[kRanked];
-  __shared__ uint32_t cand_key[kRanked];
-  __shared__ int cand_index[kRanked];
-  __shared__ int cand_n, cand_token, cand_last, cand_done;
+  __shared__ uint64_t cand[kRanked], sorted[kRanked];  // values to be ranked: key, and below it the index from the last one up
+  __shared__ int cand_n, cand_first, cand_last, cand_done;
   __shared__ struct {
     uint32_t key;
     int index;
@@ -206,6 +268,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
     const double w = TableExp2((static_cast<double>(f) - dtop) * scale, table);
     return f > cut ? w : 0.0;
   };
+  auto as_cand = [&](uint32_t key, int i) { return static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(~(lo + i)); };
+  auto key_of = [](uint64_t c) { return static_cast<uint32_t>(c >> 32); };
+  auto index_of = [](uint64_t c) { return static_cast<int>(~static_cast<uint32_t>(c)); };
   auto value_at = [&](int i) {
     const float f = ToF32(v[i]);
     return !infinite ? f : f == INFINITY ? 0.f : -INFINITY;
@@ -351,65 +416,38 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
         if (tid == 0) cand_n = 0;
         cluster.sync();
         int* const count0 = cluster.map_shared_rank(&cand_n, 0);
-        uint32_t* const key0 = cluster.map_shared_rank(cand_key, 0);
-        int* const index0 = cluster.map_shared_rank(cand_index, 0);
+        uint64_t* const cand0 = cluster.map_shared_rank(cand, 0);
         each([&](int i, float f) {
           if (bin_of(f) > b) return;
-          const int at = atomicAdd(count0, 1);
-          key0[at] = KeyOf(f);
-          index0[at] = lo + i;
+          cand0[atomicAdd(count0, 1)] = as_cand(KeyOf(f), i);
         });
         cluster.sync();
         if (rank == 0) {
-          int* const s_index = s_order;  // by rank: index, weight
           static_assert(kRanked == kSampleThreads, "a thread a value");
           const int m = cand_n;
-          if (tid < m) {
-            const uint32_t key = cand_key[tid];
-            const int index = cand_index[tid];
-            int better = 0;
-            for (int j = 0; j < m; ++j) better += cand_key[j] > key || (cand_key[j] == key && cand_index[j] < index) ? 1 : 0;
-            s_index[better] = index;
-            s_weight[better] = weight(ValueOf(key));
-          }
-          if (tid == 0) cand_token = 0x7fffffff, cand_last = 0;
-          __syncthreads();
-          const double w = tid < m ? s_weight[tid] : 0.0;
-          double up = w;  // sums up to this rank
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double t = __shfl_up_sync(0xffffffffu, up, o);
-            if (lane >= o) up += t;
-          }
-          double front = __shfl_up_sync(0xffffffffu, up, 1);
-          if (lane == 0) front = 0.0;
-          if (lane == 31) red[warp] = up;
-          __syncthreads();
-          double run = 0.0, in_all = 0.0;
-          for (int q = 0; q < kSampleWarps; ++q) {
-            if (q < warp) run += red[q];
-            in_all += red[q];
-          }
-          front += run;
-          if (by_k && tid == min(top_k, m) - 1) warp_mass[0] = run + up;
+          if (tid == 0) cand_first = kRanked, cand_last = 0;
+          const uint64_t c = SortDown(cand[tid], m, sorted);
+          const double w = tid < m ? weight(ValueOf(key_of(c))) : 0.0;
+          double in_all;
+          const double front = SumBefore(w, red, &in_all);
+          s_weight[tid] = w;
+          if (by_k && tid == min(top_k, m) - 1) warp_mass[0] = front + w;
           __syncthreads();
           const double share = by_p ? fmax(static_cast<double>(top_p) * (by_k ? warp_mass[0] : all), 1e-300) : 0.0;
           const bool reached = by_k || in_all >= share || m == a.n;  // the rough masses may have stopped short
           const bool keep = tid < m && (!by_k || tid < top_k) && (!by_p || front < share || tid == 0) && w >= least && w > 0.0;
-          const int index = tid < m ? s_index[tid] : 0;
+          if (keep) atomicMax(&cand_last, tid);
           __syncthreads();
-          if (tid < m) s_weight[tid] = keep ? w : 0.0;
-          const double kept_all = block_sum(keep ? w : 0.0, red);
+          // The kept ones by index, and the first of them whose running sum exceeds the target.
+          const uint64_t by_index = SortDown(keep ? ~(static_cast<uint64_t>(index_of(c)) << 32 | tid) : 0u, cand_last + 1, sorted);
+          const bool is = by_index != 0u;
+          const double mine = is ? s_weight[static_cast<uint32_t>(~by_index)] : 0.0;
+          double kept_all;
+          const double before = SumBefore(mine, red, &kept_all);
           const double target = (u > 0.f ? fmin(static_cast<double>(u), 1.0) : 0.0) * kept_all;
-          if (keep) {
-            double before = 0.0;  // what is kept at lower indices
-            for (int j = 0; j < m; ++j)
-              if (s_index[j] < index) before += s_weight[j];
-            if (before + w > target) atomicMin(&cand_token, index);
-            atomicMax(&cand_last, index);
-          }
-          __syncthreads();
-          if (tid == 0 && reached) a.out[row] = cand_token != 0x7fffffff ? cand_token : cand_last;  // the last one kept, where roundings leave the target out of reach
+          if (is && before + mine > target) atomicMin(&cand_first, tid);
+          const int kept_n = __syncthreads_count(is);
+          if (reached && tid == min(cand_first, kept_n - 1)) a.out[row] = static_cast<int>(~by_index >> 32);  // the last one, where roundings leave the target out of reach
           if (tid < ranks) *cluster.map_shared_rank(&cand_done, tid) = reached ? 1 : 0;
         }
         cluster.sync();
@@ -715,8 +753,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
           if (tid == 0) cand_n = 0;
           cluster.sync();
           int* const count0 = cluster.map_shared_rank(&cand_n, 0);
-          uint32_t* const key0 = cluster.map_shared_rank(cand_key, 0);
-          int* const index0 = cluster.map_shared_rank(cand_index, 0);
+          uint64_t* const cand0 = cluster.map_shared_rank(cand, 0);
           double more = 0.0;
           each([&](int i, float f) {
             const uint32_t key = KeyOf(f);
@@ -726,9 +763,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
               if (sub < s_lo && !counting) more += weight(f);
               if (sub < s_lo || sub > s_hi) return;
             }
-            const int at = atomicAdd(count0, 1);
-            key0[at] = key;
-            index0[at] = lo + i;
+            cand0[atomicAdd(count0, 1)] = as_cand(key, i);
           });
           if (by_subs && !counting) {
             above = bin_above + cluster_sum(more, red, told_mass);
@@ -737,50 +772,22 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
             cluster.sync();
           }
           if (rank == 0) {
-            // Each value's betters among them, their number and mass: the edge is the one whose betters leave room and which itself takes the last of it.
+            // From the best down: the edge is the one whose betters leave room and which itself takes the last of it.
             const int m = cand_n;
-            for (int i = tid; i < m; i += kSampleThreads) {
-              const uint32_t key = cand_key[i];
-              const int index = cand_index[i];
-              int better = 0;
-              for (int j = 0; j < m; ++j) better += cand_key[j] > key || (cand_key[j] == key && cand_index[j] < index) ? 1 : 0;
-              if (counting ? above_n + better + 1 == want_count : false) {
-                edge_s.key = key;
-                edge_s.index = index;
-              }
-              if (!counting) s_order[better] = i;
+            if (tid == 0) cand_last = -1;
+            const uint64_t c = SortDown(cand[tid], m, sorted);
+            if (!counting) {
+              double in_all;
+              const double front = SumBefore(tid < m ? weight(ValueOf(key_of(c))) : 0.0, red, &in_all);
+              if (tid < m && (above + front < want_mass || (above_n == 0 && tid == 0))) atomicMax(&cand_last, tid);
+              __syncthreads();
             }
-            __syncthreads();
-            if (!counting && warp == 0) {  // running sums by rank, 32 at a time
-              double run = above;
-              int last = 0, stayed = 0;
-              bool over = false;
-              for (int j0 = 0; j0 < m && !over; j0 += 32) {
-                const int at = j0 + lane < m ? s_order[j0 + lane] : 0;
-                const double w = j0 + lane < m ? weight(ValueOf(cand_key[at])) : 0.0;
-                double up = w;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                  const double t = __shfl_up_sync(0xffffffffu, up, o);
-                  if (lane >= o) up += t;
-                }
-                double in_front = __shfl_up_sync(0xffffffffu, up, 1);
-                if (lane == 0) in_front = 0.0;
-                const bool stays = j0 + lane < m && (run + in_front < want_mass || (above_n == 0 && j0 + lane == 0));
-                const unsigned stay = __ballot_sync(0xffffffffu, stays);
-                if (stay != 0u) last = j0 + 31 - __clz(stay);
-                over = stay != 0xffffffffu;
-                stayed += __popc(stay);
-                run += __shfl_sync(0xffffffffu, up, 31);
-              }
-              if (lane == 0) {
-                const int at = s_order[last];
-                edge_s.key = cand_key[at];
-                edge_s.index = cand_index[at];
-                edge_s.inside = stayed > 0 && (to_end || stayed < m);
-              }
+            const int last = counting ? want_count - above_n - 1 : cand_last;
+            if (tid == max(last, 0)) {
+              edge_s.key = key_of(c);
+              edge_s.index = index_of(c);
+              edge_s.inside = last >= 0 && (counting || to_end || last + 1 < m);
             }
-            if (counting && tid == 0) edge_s.inside = true;
             __syncthreads();
             if (tid > 0 && tid < ranks) {
               cluster.map_shared_rank(&edge_s, tid)->key = edge_s.key;
