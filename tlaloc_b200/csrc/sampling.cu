@@ -14,10 +14,14 @@
 //   3  where the bins from the largest value down to the edge hold no more than 512 values, as they mostly do: these go to one CTA, which ranks them, a thread each, and
 //      finds both edges and the token among them
 //   Otherwise, per edge: the exact count and mass above the bin that it lies in; the bin's values go to one CTA, which ranks them and finds the edge.  Rough masses
-//      (a bin's count times its middle w) only say where to look: the exact ones decide, and move on to a neighbouring bin if they must.  A bin with more values than a CTA ranks is halved by
-//      value, over and over (equal logits by the thousand).  Then
+//      (a bin's count times its middle w) only say where to look: the exact ones decide, and move on to a neighbouring bin if they must.  A bin with more values than a CTA
+//      ranks is counted again in 512 parts, of which one CTA takes those around the edge; where these hold too many as well (equal logits by the thousand) it is halved
+//      by value, over and over.  Then
 //   4  the mass that is kept, by warp, and the draw, in the one warp whose stretch it falls into
-// Without top-k and top-p there are passes 1 and 4 alone, which the f64 units bound: nine operations an exponential.
+//
+// Not bound by HBM but by the passes' instructions (some 15 to 40 a value) and the steps that the cluster takes together (1 to 2 us each).  A row of 128256 f32 values: passes 1 and 2
+// 2.5 and 5.5 us, joining the bins 4, gathering 5, ranking 3 to 7; an edge among more than 512 values 25 beside.  Temperature alone takes passes 1 and 4, bound by the f64
+// units (nine operations an exponential): 512 rows of 32768 bf16 values 53 us, 128 rows of 128256 f32 values 56; with all filters 154.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -76,7 +80,8 @@ __device__ __forceinline__ double TableExp2(double t, const double* table)
 }
 
 // The block's values from the largest down, one a thread, of its first n threads; zeros come last.  No other value twice.  Few are ranked by counting the larger ones of all, more
-// sorted by a bitonic network (strides below 32 through shuffles): 64 values take some 700 cycles counted and 1500 sorted, 512 take 12000 and 3000.
+// sorted by a bitonic network (strides below 32 through shuffles).  One row of 128256
+// values, 50 ranked: 28.3 us counted, 32.0 sorted; two rows of 151937, some 500 ranked: 52.9 and 44.1.
 constexpr int kCounted = 128;
 __device__ __noinline__ uint64_t SortDown(uint64_t v, int n, uint64_t* buffer)
 {
@@ -945,6 +950,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) SampleKernel(const __grid_c
 }
 
 constexpr int kPartBytes = 160 * 1024;  // of a row that a CTA keeps
+constexpr int kLeastPart = 2048;        // values that a CTA of a small batch takes
 
 cudaError_t PrepareSample()
 {
@@ -973,9 +979,17 @@ extern "C" int tlaloc_b200_sample(const void* logits, int64_t ld, int32_t dtype,
   if (rows == 0) return kOk;
   cudaError_t e = PrepareSample();
   if (e != cudaSuccess) return CudaFail("SAMPLE set-up", e);
-  // A CTA takes 16384 values, 64 KB of f32: three of them fit an SM, and few rows of a large vocabulary still spread over eight.
-  int ranks = 1;
-  while (ranks < kMaxRanks && static_cast<long long>(ranks) * 16384 < n) ranks *= 2;
+  // A CTA takes 16384 values (64 KB of f32: two share an SM), fewer while all parts of the batch run at once.  Of 32768 values with all filters: one row 28.8 us in parts of
+  // 16384, 21.4 of 8192, 18.2 of 4096; 32 rows 46.6, 34.9, 31.4; one row of 4099 17.6 in one part, 16.9 in 2048s.  Past what runs at once the parts' common
+  // steps cost more than they spread: 256 rows of 65536 146 us in 16384s, 200 in 8192s, 177 in 32768s.
+  auto ranks_of = [&](int part) {
+    int ranks = 1;
+    while (ranks < kMaxRanks && static_cast<long long>(ranks) * part < n) ranks *= 2;
+    return ranks;
+  };
+  int part = kLeastPart;
+  while (part < 16384 && static_cast<long long>(rows) * ranks_of(part) > 2 * 148) part *= 2;
+  const int ranks = ranks_of(part);
   SampleArgs a = {logits, ld, uniforms, temperature, top_k, top_p, min_p, temperature_all, top_p_all, min_p_all, top_k_all, out, n, 0, 0};
   a.per = ((n + ranks - 1) / ranks + 7) / 8 * 8;
   const size_t bytes = static_cast<size_t>(a.per) * DtypeBytes(dtype);

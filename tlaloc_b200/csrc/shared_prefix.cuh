@@ -18,7 +18,6 @@ struct PrefixPlan {
   int max_len;        // positions that a prefix table holds
   int unit_rows, tile;
   int grid;           // CTAs of the record kernel
-  int min_run;        // tiles, at least, of a CTA's run
   int max_blocks;     // blocks of records that there is room for
 };
 
@@ -49,7 +48,7 @@ class PrefixLine {
       units = unit_end_;
     }
     if (p.G > 32) Load(0, 0, 0);
-    run = max((total + p.grid - 1) / p.grid, p.min_run);
+    run = max((total + p.grid - 1) / p.grid, 1);  // short ones too: a tile a CTA beats four (two rows of 500 positions 18.8 us, 22.7)
   }
 
   // The group that holds tile `at` of the line (by_row false), or query row `at` (by_row true); false if there is none.

@@ -10,8 +10,10 @@
 //                   one after the other, 85 cycles each: 16 of 16 positions by one warp alone were late)
 //   MMA lane        in turn for the streams: O += P(i) V(i), S(i + 1)
 //   sixteen warps   softmax, a stream's by eight: two threads a pair, each half of its scores; before that the queries into shared memory, at the end the records
-// What bounds it where many pairs share a prefix is shared memory, which feeds both operands of S and one of O: 64-key scores in two places, which spare the softmax its
-// waits, read the queries twice as often and were no faster.
+// What bounds it where many pairs share a prefix: a step of 256 pairs x 128 keys takes 4600 cycles, though its products need 2544 and its exponentials 2048, and HBM is not
+// awaited (tables whose pages all lie in L2 are 6 % faster).  Products that read both operands from shared memory hold up the barriers' arrivals and the softmax's stores by
+// hundreds of cycles.  128 rows of 64 heads over 32768 positions: 159 us, 864 TFLOP/s (177 under a
+// sustained load's clocks); 64 rows of 32 heads (f32 queries) over 8192 31 us; two rows over 500 11: a segment's start and end, 8 us, are what short prefixes take.
 // An f32 query enters as two bf16 parts.  Where the result is f32 the weights do as well (2^-17 of them is lost); for a bf16 result one part is enough: what is lost
 // (2^-9 of each weight, at random) is less than the result's own rounding.
 // e4m3fn rows: f16 holds every value, so both products are f16 x f16 (queries and weights as f16 parts), and the three warps that fill the ring read the rows with plain
