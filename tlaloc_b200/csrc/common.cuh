@@ -182,11 +182,11 @@ cudaError_t LaunchInt8GemmI8(const void* x, int x_dtype, const int8_t* codes, co
 // The quantizer alone: the planes of x [m, k] into `planes` (Int8GemmI8ScratchBytes(m, k) bytes).
 cudaError_t LaunchQuantizeRowsI8(const void* x, int x_dtype, void* planes, int m, int k, cudaStream_t st);
 // The slice kernels of paged attention (paged_attention.cu) without their merge: records f32 [splits, R, H, D + 2] = {max, sum, acc[D]}; *slice positions a
-// slice, *slices of them; a row's live ones are [0, ceil(len / slice)).  The checks, and their messages under the name `op`, are the operator's own.
+// slice (generic_slice in the generic kernel, 256 or more in the others), *slices of them; a row's live ones are [0, ceil(len / slice)).  The checks, and their messages under the name `op`, are the operator's own.
 int LaunchPagedSlices(const char* op, const void* query, int32_t q_dtype, const void* key_cache, const void* value_cache, int32_t kv_dtype,
                       const int32_t* block_tables, const int32_t* seq_lens, float* records, int32_t splits, int32_t num_rows, int32_t num_heads, int32_t head_dim,
-                      int32_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t max_blocks_per_seq, int32_t num_tables, float scale, cudaStream_t st,
-                      int32_t* slice, int32_t* slices);
+                      int32_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t max_blocks_per_seq, int32_t num_tables, float scale, int32_t generic_slice,
+                      cudaStream_t st, int32_t* slice, int32_t* slices);
 bool EncodeKvPoolMap(::CUtensorMap_st* map, const void* base, int head_dim, int kv_heads, unsigned long long positions, int elem_bytes);
 
 // The activation planes of the int8 tensor-core projection: row m of x as q = rint(x / s[m]) = 256 hi + lo with s[m] the

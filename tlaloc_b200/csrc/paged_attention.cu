@@ -1679,8 +1679,8 @@ int ParseCall(const char* op, const void* query, int32_t q_dtype, const void* ke
   return kOk;
 }
 
-// The slice kernels of a parsed call: fills in the slices that they use.
-int LaunchSlices(const char* op, PaParams& p, int32_t q_dtype, int32_t kv_dtype, int32_t splits, cudaStream_t st)
+// The slice kernels of a parsed call: fills in the slices that they use (the generic kernel's: `generic_slice` positions).
+int LaunchSlices(const char* op, PaParams& p, int32_t q_dtype, int32_t kv_dtype, int32_t splits, int generic_slice, cudaStream_t st)
 {
   const int ctx = p.M * p.bs;
   // The tensor-core kernel copies K/V rows in 16-byte pieces: pools that start off a 16-byte boundary (a slice of a
@@ -1693,10 +1693,10 @@ int LaunchSlices(const char* op, PaParams& p, int32_t q_dtype, int32_t kv_dtype,
   const bool f8 = kv_dtype == TLALOC_B200_F8E4M3FN;
   const bool mma = (kv_dtype == TLALOC_B200_BF16 || (f8 && !f8_generic)) && (p.D == 64 || p.D == 128) && p.NQ <= kMmaQ &&
                    p.keep == nullptr && (f8 ? p.bs >= 16 : p.bs >= 8) && Aligned16(p.kc) && Aligned16(p.vc);
-  // Slice length: the preferred one (tensor-core kernel) or 256, stretched until `splits` slices cover the context.
+  // Slice length: the preferred one (tensor-core kernel) or the generic one, stretched until `splits` slices cover the context.
   const bool from_window = p.window > 0 && p.window < ctx && p.rpt == 1;  // rows that share a table have windows in different places: all slices are launched for them
   const int seen = from_window ? p.window : ctx;
-  int slice = mma ? PreferredSlice(seen, from_window, p.Tb, p.Hkv, f8) : 256;
+  int slice = mma ? PreferredSlice(seen, from_window, p.Tb, p.Hkv, f8) : generic_slice;
   if (static_cast<int64_t>(slice) * splits < ctx) slice = (ctx + splits - 1) / splits;
   if (mma) slice = std::min((slice + 15) / 16 * 16, 8192);
   if (static_cast<int64_t>(slice) * splits < ctx) {
@@ -1739,13 +1739,13 @@ int LaunchSlices(const char* op, PaParams& p, int32_t q_dtype, int32_t kv_dtype,
 
 int LaunchPagedSlices(const char* op, const void* query, int32_t q_dtype, const void* key_cache, const void* value_cache, int32_t kv_dtype,
                       const int32_t* block_tables, const int32_t* seq_lens, float* records, int32_t splits, int32_t num_rows, int32_t num_heads, int32_t head_dim,
-                      int32_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t max_blocks_per_seq, int32_t num_tables, float scale, cudaStream_t st,
-                      int32_t* slice, int32_t* slices)
+                      int32_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t max_blocks_per_seq, int32_t num_tables, float scale, int32_t generic_slice,
+                      cudaStream_t st, int32_t* slice, int32_t* slices)
 {
   PaParams p;
   int rc = ParseCall(op, query, q_dtype, key_cache, value_cache, kv_dtype, block_tables, seq_lens, nullptr, 0, records, TLALOC_B200_F32, nullptr, records, splits,
                      num_rows, num_heads, head_dim, num_blocks, block_size, num_kv_heads, max_blocks_per_seq, num_tables, scale, 0, &p);
-  if (rc == kOk) rc = LaunchSlices(op, p, q_dtype, kv_dtype, splits, st);
+  if (rc == kOk) rc = LaunchSlices(op, p, q_dtype, kv_dtype, splits, generic_slice, st);
   if (rc != kOk) return rc;
   *slice = p.slice;
   *slices = p.S;
@@ -1787,7 +1787,7 @@ extern "C" int tlaloc_b200_paged_attention(const void* query, int32_t q_dtype, c
     CountLaunches(1);
     return kOk;
   }
-  rc = LaunchSlices(op, p, q_dtype, kv_dtype, splits, st);
+  rc = LaunchSlices(op, p, q_dtype, kv_dtype, splits, 256, st);
   if (rc != kOk) return rc;
   cudaError_t e = cudaSuccess;
   const unsigned cgrid = static_cast<unsigned>((p.R * p.H + kCombineThreads / 32 - 1) / (kCombineThreads / 32));

@@ -340,6 +340,7 @@ cudaError_t LaunchMerge(const MergeArgs& m, cudaStream_t st)
 // Host side.
 
 constexpr int kTiledGrid = 2 * 148;
+constexpr int kLeastOwnSlice = 32;
 
 size_t TiledSmem(int D) { return sizeof(float) * ((kPairs + 2 * kTileKeys) * ((D + 3) / 4 * 4 + 4) + kPairs * (kTileKeys + 1)); }
 
@@ -400,7 +401,21 @@ long long LineTiles(int rows, int heads, int kv_heads, int prefixes, int unit_ro
 {
   return (RecordBlocks(rows, heads, kv_heads, prefixes, unit_rows, 0) + 1) * ((max_len + tile - 1) / tile);
 }
-int OwnSlices(int max_blocks, int block_size) { return static_cast<int>((static_cast<long long>(max_blocks) * block_size + 255) / 256); }
+// Positions of an own slice of the generic kernel: 256, halved (down to 32) while a launch has fewer than 16 CTAs an SM.  Its CTAs spend their time waiting, a position after the
+// other.  All three launches, 8 KV heads, up to 1024 own positions, slices of 256 / halved up to 2 / 6 / 16 CTAs an SM: one row of an f32 pool 131 / 51 / 51 / 51 us, 4 rows
+// 143 / 65 / 56 / 55, 16 rows 228 / 227 / 140 / 103, 64 rows 273 / 271 / 273 / 262; heads of 80 in a bf16 pool 107 / 41 / 40 / 41 to 188 / 188 / 188 / 179.
+int OwnSlice(int rows, int kv_heads, long long ctx)
+{
+  int slice = 256;
+  while (slice > kLeastOwnSlice && static_cast<long long>(rows) * kv_heads * ((ctx + slice - 1) / slice) < 16 * 148) slice /= 2;
+  return slice;
+}
+int OwnSlices(int rows, int kv_heads, int max_blocks, int block_size)
+{
+  const long long ctx = static_cast<long long>(max_blocks) * block_size;
+  const int slice = OwnSlice(rows, kv_heads, ctx);
+  return static_cast<int>((ctx + slice - 1) / slice);
+}
 
 }  // namespace
 }  // namespace tlaloc_b200
@@ -414,7 +429,7 @@ extern "C" size_t tlaloc_b200_shared_prefix_scratch_bytes(int32_t num_rows, int3
   // Whichever record kernel takes the call: that hangs on types and addresses too.
   const size_t tiled = RecordBytes(RecordBlocks(num_rows, num_heads, num_kv_heads, num_prefixes, kPairs, kTiledGrid), kPairs, head_dim);
   const size_t tc = head_dim <= 128 ? RecordBytes(RecordBlocks(num_rows, num_heads, num_kv_heads, num_prefixes, kPrefixTcPairs, kPrefixTcGrid), kPrefixTcPairs, head_dim) : 0;
-  return std::max(tiled, tc) + tlaloc_b200_paged_attention_scratch_bytes(num_rows, num_heads, head_dim, OwnSlices(max_blocks_per_seq, block_size));
+  return std::max(tiled, tc) + tlaloc_b200_paged_attention_scratch_bytes(num_rows, num_heads, head_dim, OwnSlices(num_rows, num_kv_heads, max_blocks_per_seq, block_size));
 }
 
 extern "C" int tlaloc_b200_shared_prefix_attention(const void* query, int32_t q_dtype, const void* key_cache, const void* value_cache, int32_t kv_dtype,
@@ -436,7 +451,7 @@ extern "C" int tlaloc_b200_shared_prefix_attention(const void* query, int32_t q_
     return Fail(kInvalid, "%s: scratch must be 32-byte aligned and hold %zu bytes (got %zu)", op, need, scratch_bytes);
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int own_slices = OwnSlices(max_blocks_per_seq, block_size);
+  const int own_slices = OwnSlices(num_rows, num_kv_heads, max_blocks_per_seq, block_size);
   PrefixArgs a = {};
   a.plan.lens = prefix_lens;
   a.plan.starts = row_starts;
@@ -471,7 +486,8 @@ extern "C" int tlaloc_b200_shared_prefix_attention(const void* query, int32_t q_
   MergeArgs m = {};
   // The own part first: its checks are those of all the operands that both parts share.
   int rc = LaunchPagedSlices(op, query, q_dtype, key_cache, value_cache, kv_dtype, block_tables, seq_lens, own, own_slices, num_rows, num_heads, head_dim,
-                             num_blocks, block_size, num_kv_heads, max_blocks_per_seq, num_tables, scale, st, &m.slice, &m.slices);
+                             num_blocks, block_size, num_kv_heads, max_blocks_per_seq, num_tables, scale,
+                             OwnSlice(num_rows, num_kv_heads, static_cast<long long>(max_blocks_per_seq) * block_size), st, &m.slice, &m.slices);
   if (rc != kOk) return rc;
   cudaError_t e = PrepareSharedPrefix();
   if (e != cudaSuccess) return CudaFail("SHARED_PREFIX_ATTENTION set-up", e);
