@@ -131,6 +131,16 @@ def test_groups(lens, rows, starts, pool):
     c.check(got, lse)
 
 
+@pytest.mark.parametrize("rows", [1, 3, 16, 150])
+@pytest.mark.parametrize("pool,D", [(F32, 128), (BF16, 80), (F8, 256), (BF16, 128)])
+def test_own_lengths_around_slices(pool, D, rows):
+    """Own parts in slices of 32 to 256 positions, by how many rows there are."""
+    lens = [0, 1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 511, 512, 513, 1000]
+    c = Case([100], rows, [lens[(5 * r + rows) % len(lens)] for r in range(rows)], H=4, Hkv=2, D=D, pool=pool, query=F32, seed=rows, wide=1024 // 16)
+    out, lse = c.run(out_dtype=F32, return_lse=True)
+    c.check(out, lse)
+
+
 def test_long_prefix():
     c = Case([20000], 24, 100, H=16, Hkv=2)
     c.check(c.run(out_dtype=F32), rows=[0, 11, 23])
